@@ -5,6 +5,7 @@
 #include <torch/extension.h>
 
 #include "host/recall_dispatch.h"
+#include "kernels/generation.h"
 #include "kernels/launchers.h"
 
 namespace {
@@ -399,6 +400,90 @@ void sparse_mla(const Tensor& q, const Tensor& kv, const Tensor& ids, double sca
   } else {
     b200::launch_sparse_mla_split(a, int(splits), sp, stream());
   }
+}
+
+// --------------------------------------------- continuations of one history
+// q [B,T,H,576] over prefix [P,576] plus the visible rows of tail [B,S,576].
+void shared_prefix_mla(const Tensor& q, const Tensor& prefix, const c10::optional<Tensor>& tail,
+                       const c10::optional<Tensor>& tail_lens, double scale, Tensor& out,
+                       const c10::optional<Tensor>& lse) {
+  CHECK_CUDA(q); CHECK_CUDA(prefix); CHECK_CUDA(out);
+  CHECK_DTYPE(q, torch::kBFloat16); CHECK_DTYPE(prefix, torch::kBFloat16); CHECK_DTYPE(out, torch::kBFloat16);
+  TORCH_CHECK(q.dim() == 4 && q.size(3) == 576 && q.is_contiguous(), "shared_prefix_mla: q [B,T,H,576]");
+  TORCH_CHECK(out.dim() == 4 && out.is_contiguous() && out.size(0) == q.size(0) && out.size(1) == q.size(1) &&
+                  out.size(2) == q.size(2) && out.size(3) == 512, "shared_prefix_mla: out [B,T,H,512]");
+  auto rows_ok = [](const Tensor& t) {  // records of 576 dims on 16-byte boundaries
+    bool ok = t.size(-1) == 576 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+    if (t.numel() == 0) return ok;
+    ok = ok && t.stride(-1) == 1;
+    for (int64_t d = 0; d + 1 < t.dim(); ++d) ok = ok && (t.size(d) == 1 || (t.stride(d) >= 0 && t.stride(d) % 8 == 0));
+    return ok;
+  };
+  TORCH_CHECK(prefix.dim() == 2 && rows_ok(prefix) && prefix.size(0) < (int64_t(1) << 31),
+              "shared_prefix_mla: prefix [P,576], rows 16-byte aligned");
+  TORCH_CHECK(prefix.device() == q.device() && out.device() == q.device(), "shared_prefix_mla: one device");
+  c10::cuda::CUDAGuard g(q.device());
+  b200::PrefixMLAArgs a{};
+  a.q = cptr<__nv_bfloat16>(q); a.prefix = cptr<__nv_bfloat16>(prefix); a.out = ptr<__nv_bfloat16>(out);
+  a.B = q.size(0); a.T = q.size(1); a.H = q.size(2); a.P = prefix.size(0); a.scale = float(scale);
+  a.ld_prefix = prefix.size(0) > 1 ? prefix.stride(0) : 576;
+  a.err = err_ptr(q);
+  if (tail && tail->defined()) {
+    CHECK_DTYPE((*tail), torch::kBFloat16);
+    TORCH_CHECK(tail->dim() == 3 && tail->size(0) == q.size(0) && rows_ok(*tail) && tail->device() == q.device(),
+                "shared_prefix_mla: tail [B,S,576], rows 16-byte aligned");
+    a.tail = cptr<__nv_bfloat16>(*tail);
+    a.S = tail->size(1); a.ld_batch = tail->stride(0); a.ld_tail = tail->stride(1);
+    if (tail_lens && tail_lens->defined()) {
+      CHECK_DTYPE((*tail_lens), torch::kInt32);
+      TORCH_CHECK(tail_lens->is_contiguous() && tail_lens->dim() == 1 && tail_lens->size(0) == q.size(0) &&
+                      tail_lens->device() == q.device(), "shared_prefix_mla: tail_lens [B] int32");
+      a.tail_lens = cptr<int>(*tail_lens);
+    }
+  }
+  if (lse && lse->defined()) {
+    CHECK_DTYPE((*lse), torch::kFloat32);
+    TORCH_CHECK(lse->is_contiguous() && lse->numel() == q.size(0) * q.size(1) * q.size(2), "shared_prefix_mla: lse");
+    a.lse = ptr<float>(*lse);
+  }
+  b200::launch_shared_prefix_mla(a, stream());
+}
+
+void sample_tokens(const Tensor& logits, const Tensor& u, const c10::optional<Tensor>& temperature,
+                   const c10::optional<Tensor>& top_k, const c10::optional<Tensor>& top_p,
+                   const c10::optional<Tensor>& min_p, double temperature0, int64_t top_k0, double top_p0,
+                   double min_p0, Tensor& tokens, Tensor& logprobs) {
+  CHECK_CUDA(logits); CHECK_DTYPE(u, torch::kFloat32); CHECK_DTYPE(tokens, torch::kInt64);
+  CHECK_DTYPE(logprobs, torch::kFloat32);
+  TORCH_CHECK(logits.scalar_type() == torch::kFloat32 || logits.scalar_type() == torch::kBFloat16,
+              "sample_tokens: logits FP32 or BF16");
+  TORCH_CHECK(logits.dim() == 2 && logits.size(1) >= 1 && (logits.size(1) == 1 || logits.stride(1) == 1) &&
+                  logits.stride(0) >= 0, "sample_tokens: logits [R,V], contiguous in the vocabulary");
+  const int64_t R = logits.size(0);
+  auto per_row = [&](const Tensor& t, const char* what) {
+    TORCH_CHECK(t.dim() == 1 && t.size(0) == R && t.is_contiguous() && t.device() == logits.device(),
+                "sample_tokens: ", what, " must be a contiguous [R] tensor on the logits' device");
+  };
+  per_row(u, "u"); per_row(tokens, "tokens"); per_row(logprobs, "logprobs");
+  c10::cuda::CUDAGuard g(logits.device());
+  b200::SampleArgs a{};
+  a.logits = logits.data_ptr(); a.bf16 = logits.scalar_type() == torch::kBFloat16; a.ld = logits.stride(0);
+  a.R = R; a.V = logits.size(1); a.u = cptr<float>(u);
+  auto floats = [&](const c10::optional<Tensor>& t, const char* what) -> const float* {
+    if (!t || !t->defined()) return nullptr;
+    CHECK_DTYPE((*t), torch::kFloat32);
+    per_row(*t, what);
+    return cptr<float>(*t);
+  };
+  a.temperature = floats(temperature, "temperature"); a.top_p = floats(top_p, "top_p"); a.min_p = floats(min_p, "min_p");
+  if (top_k && top_k->defined()) {
+    CHECK_DTYPE((*top_k), torch::kInt32);
+    per_row(*top_k, "top_k");
+    a.top_k = cptr<int>(*top_k);
+  }
+  a.temperature0 = float(temperature0); a.top_p0 = float(top_p0); a.min_p0 = float(min_p0); a.top_k0 = int(top_k0);
+  a.tokens = ptr<int64_t>(tokens); a.logprobs = ptr<float>(logprobs);
+  b200::launch_sample_tokens(a, stream());
 }
 
 Tensor topk_trace(int64_t row) {
@@ -891,6 +976,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("diag") = py::none());
   m.def("topk", &topk);
   m.def("sparse_mla", &sparse_mla);
+  m.def("shared_prefix_mla", &shared_prefix_mla);
+  m.def("sample_tokens", &sample_tokens);
   m.def("sparse_mla_scratch_bytes", &sparse_mla_scratch_bytes);
   m.def("sparse_mla_trace", &sparse_mla_trace);
   m.def("topk_trace", &topk_trace);

@@ -12,6 +12,7 @@ import math
 import torch
 
 from . import reference
+from .generation import sample_tokens, shared_prefix_mla  # noqa: F401
 from .native import check_errors, error_word, lib  # noqa: F401
 
 FP8 = torch.float8_e4m3fn

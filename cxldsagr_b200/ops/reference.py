@@ -273,6 +273,73 @@ def sparse_mla_lse(q, kv, indices, scale, value_dim=512):
     return out, lse
 
 
+def shared_prefix_mla(q, prefix, tail, tail_lens, scale, value_dim=512):
+    """q [B,H,D] or [B,T,H,D] over prefix [P,D] and the visible rows of tail [B,S,D]; (out, lse)."""
+    q4 = q if q.dim() == 4 else q.unsqueeze(1)
+    B, T, H, _ = q4.shape
+    out = torch.zeros((B, T, H, value_dim), dtype=torch.float32, device=q.device)
+    lse = torch.full((B, T, H), -torch.inf, dtype=torch.float32, device=q.device)
+    for b in range(B):
+        n = 0 if tail is None else tail.shape[1] if tail_lens is None else int(tail_lens[b])
+        if n < 0 or (tail is not None and n > tail.shape[1]):
+            raise IndexError("tail length outside the tail")
+        for t in range(T):
+            rec = prefix.float()
+            seen = max(0, n - (T - 1 - t))
+            if seen:
+                rec = torch.cat((rec, tail[b, :seen].float()))
+            if not rec.shape[0]:
+                continue
+            logits = q4[b, t].float() @ rec.T * scale
+            lse[b, t] = torch.logsumexp(logits, -1)
+            out[b, t] = logits.softmax(-1) @ rec[:, :value_dim]
+    return out.to(q.dtype).reshape(*q.shape[:-1], value_dim), lse.reshape(q.shape[:-1])
+
+
+# -------------------------------------------------------------- sampling
+SAMPLE_FIXED = float(2 ** 36)  # sampling masses are whole multiples of 2^-36 of the best token's weight
+
+
+def sample_tokens(logits, u, temperature, top_k, top_p, min_p):
+    """Token and log-probability per row; the rule is stated at :func:`..ops.sample_tokens`."""
+    R, V = logits.shape
+    dev = logits.device
+    tokens = torch.full((R,), -1, dtype=torch.int64, device=dev)
+    logprobs = torch.full((R,), -torch.inf, dtype=torch.float32, device=dev)
+
+    def at(v, r):
+        return v[r].item() if torch.is_tensor(v) else torch.tensor(v).item()
+
+    for r in range(R):
+        x = logits[r].float()
+        x = torch.where(torch.isnan(x), -torch.inf, x)
+        T, k, p, mp = at(temperature, r), int(at(top_k, r)), at(top_p, r), at(min_p, r)
+        ranked, order = torch.sort(x, descending=True, stable=True)
+        if ranked[0] == -torch.inf:
+            continue
+        if not T > 0:
+            tokens[r], logprobs[r] = order[0], 0.0
+            continue
+        d = torch.where(ranked == ranked[0], 0.0, (ranked - ranked[0]) / T)
+        w = torch.where(ranked == -torch.inf, 0.0, torch.exp(d))
+        mass = (w * SAMPLE_FIXED).long()
+        n = V if k <= 0 else min(k, V)
+        if p < 1:
+            want = p * mass[:n].sum().double()
+            n = max(1, int(((mass.cumsum(0) - mass)[:n].double() < want).sum()))
+        if mp == mp:
+            n = max(1, min(n, int((w >= mp).sum())))
+        ids, by_id = torch.sort(order[:n])
+        cum = mass[:n][by_id].cumsum(0)
+        total = cum[-1]
+        want = torch.nan_to_num(u[r].double(), nan=0.0) * total.double()
+        target = min(max(int(want.floor().clamp(0, 2.0**62)), 0), int(total) - 1)
+        j = int((cum <= target).sum())
+        tokens[r] = ids[j]
+        logprobs[r] = d[by_id[j]].double() - torch.log(total.double() / SAMPLE_FIXED)
+    return tokens, logprobs
+
+
 # ------------------------------------------------------------------- moe
 def route_experts(hidden, gate_weight, correction_bias, cfg):
     """Sigmoid scores; bias-corrected group choice (top-2 sum per group, top groups), top-k experts.

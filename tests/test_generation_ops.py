@@ -1,0 +1,490 @@
+"""Shared-prefix MLA and token sampling against their definitions in 64 bits."""
+
+import math
+
+import pytest
+import torch
+
+from cxldsagr_b200 import ops
+from cxldsagr_b200.ops import reference as ref
+
+SCALE = 0.1352
+gpu = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _check_device_errors():
+    yield
+    if torch.cuda.is_available():
+        torch.cuda.synchronize()
+        ops.check_errors("cuda")
+
+
+# ------------------------------------------------------- shared-prefix MLA
+def prefix_oracle(q, prefix, tail, lens, scale, dv):
+    """(out, lse, sum_j p_j |v_j|, max_j scale |q| . |k_j|) in float64, one query at a time."""
+    q4 = (q if q.dim() == 4 else q[:, None]).double()
+    B, T, H, D = q4.shape
+    out = torch.zeros(B, T, H, dv, dtype=torch.float64, device=q.device)
+    mag = torch.zeros_like(out)
+    lse = torch.full((B, T, H), -math.inf, dtype=torch.float64, device=q.device)
+    size = torch.zeros_like(lse)
+    for b in range(B):
+        for t in range(T):
+            rec = prefix.double()
+            if tail is not None:
+                seen = max(0, int(lens[b]) - (T - 1 - t))
+                rec = torch.cat((rec, tail[b, :seen].double()))
+            if rec.shape[0] == 0:
+                continue
+            s = scale * (q4[b, t] @ rec.T)
+            w = torch.softmax(s, -1)
+            lse[b, t] = torch.logsumexp(s, -1)
+            out[b, t] = w @ rec[:, :dv]
+            mag[b, t] = w @ rec[:, :dv].abs()
+            size[b, t] = (scale * (q4[b, t].abs() @ rec.abs().T)).amax(-1)
+    shape = q.shape[:-1]
+    return out.reshape(*shape, dv), lse.reshape(shape), mag.reshape(*shape, dv), size.reshape(shape)
+
+
+def check_prefix(q, prefix, tail, lens, got, lse, scale=SCALE):
+    dv = got.shape[-1]
+    full = lens if lens is not None or tail is None else [tail.shape[1]] * q.shape[0]
+    want, wlse, mag, size = prefix_oracle(q, prefix, tail, full, scale, dv)
+    # The probabilities and the output are rounded to BF16 once each (2^-9 relative): |error| <=
+    # 2^-9 sum p|v| + 2^-9 |out| <= 2^-8 sum p|v|.  The scores are FP32 sums of 576 exact products, each
+    # step within 2^-23 of the running sum (a random walk of ~sqrt(576) steps is taken as 32): their error
+    # adds twice that (numerator and denominator) relative to the same sum.
+    score_err = 32 * 2.0**-23 * size
+    bound = (2.0**-8 + 2 * score_err[..., None] + 2.0**-20) * mag + 1e-30
+    err = (got.double() - want).abs()
+    assert torch.isfinite(got).all()
+    assert (err <= bound).all(), f"output off by {(err / bound).max().item():.2f} of its bound"
+    if lse is not None:
+        assert torch.equal(torch.isinf(lse), torch.isinf(wlse))
+        ok = ~torch.isinf(wlse)
+        tol = score_err + 2.0**-21 * (1 + wlse.abs())
+        assert ((lse.double() - wlse).abs()[ok] <= tol[ok]).all()
+
+
+def prefix_inputs(B, T, H, P, S, device, D=576, seed=0, room=0):
+    g = torch.Generator().manual_seed(seed)
+    q = (torch.randn(B, T, H, D, generator=g) * 0.5).bfloat16().to(device)
+    prefix = torch.randn(P, D, generator=g).bfloat16().to(device)
+    tail = torch.randn(B, S + room, D, generator=g).bfloat16().to(device)[:, :S]
+    return q, prefix, tail
+
+
+GPU_SHAPES = [  # B, T, H, P, S, lens
+    (1, 1, 128, 1, 1, [1]),
+    (1, 1, 128, 1, 1, [0]),
+    (2, 1, 128, 0, 3, [0, 3]),          # no history; one row sees nothing
+    (3, 1, 128, 64, 64, [64, 1, 0]),
+    (2, 1, 128, 63, 65, [65, 64]),
+    (2, 1, 128, 65, 130, [129, 128]),
+    (5, 1, 128, 1999, 33, [11, 14, 17, 20, 23]),
+    (2, 3, 128, 100, 7, [7, 1]),        # the second continuation's first query tokens see only the history
+    (2, 4, 128, 0, 4, [4, 2]),          # ... or nothing at all
+    (9, 1, 16, 333, 70, [70, 0, 1, 63, 64, 65, 2, 33, 69]),
+    (7, 1, 20, 129, 5, [5, 4, 3, 2, 1, 0, 5]),
+    (3, 2, 64, 511, 9, [9, 8, 2]),
+    (2, 1, 1, 200, 4, [4, 1]),
+    (2, 1, 200, 77, 66, [66, 65]),      # more heads than a row tile
+    (2, 1, 256, 300, 10, [10, 3]),
+    (1, 1, 128, 20011, 2, [1]),         # a long history split over the SMs
+    (80, 1, 128, 257, 5, None),         # more row tiles than SM pairs
+]
+
+
+@gpu
+@pytest.mark.parametrize("B,T,H,P,S,lens", GPU_SHAPES)
+def test_shared_prefix_mla_gpu(B, T, H, P, S, lens):
+    q, prefix, tail = prefix_inputs(B, T, H, P, S, "cuda", room=2)
+    lt = None if lens is None else torch.tensor(lens, dtype=torch.int32, device="cuda")
+    out, lse = ops.shared_prefix_mla(q, prefix, tail, lt, SCALE, return_lse=True)
+    check_prefix(q, prefix, tail, lens, out, lse)
+    if T == 1:  # the three-dimensional form is the same call
+        o3 = ops.shared_prefix_mla(q[:, 0], prefix, tail, lt, SCALE)
+        assert torch.equal(o3, out[:, 0])
+
+
+@gpu
+def test_shared_prefix_mla_no_tail_and_repeats():
+    q, prefix, _ = prefix_inputs(3, 1, 128, 700, 1, "cuda", seed=1)
+    out, lse = ops.shared_prefix_mla(q, prefix, None, None, SCALE, return_lse=True)
+    check_prefix(q, prefix, None, None, out, lse)
+    for _ in range(3):
+        again, lse2 = ops.shared_prefix_mla(q, prefix, None, None, SCALE, return_lse=True)
+        assert torch.equal(again, out) and torch.equal(lse2, lse)
+    empty = ops.shared_prefix_mla(q[:0], prefix, None, None, SCALE)
+    assert empty.shape == (0, 1, 128, 512)
+
+
+@gpu
+@pytest.mark.parametrize("H", [128, 16])
+def test_shared_prefix_mla_unseen_rows_hold_anything(H):
+    """Tail rows past the visible length (and another continuation's rows) may be NaN or infinite."""
+    q, prefix, tail = prefix_inputs(6, 1, H, 130, 70, "cuda", seed=2)
+    lens = [0, 1, 69, 64, 35, 70]
+    clean = ops.shared_prefix_mla(q, prefix, tail, torch.tensor(lens, dtype=torch.int32, device="cuda"), SCALE)
+    dirty = tail.clone()
+    for b, n in enumerate(lens):
+        dirty[b, n:] = float("nan") if b % 2 else float("inf")
+    dirty[5] = float("nan")  # continuation 5 is poisoned altogether; the others must not notice
+    got = ops.shared_prefix_mla(q, prefix, dirty, torch.tensor(lens, dtype=torch.int32, device="cuda"), SCALE)
+    assert torch.equal(got[:5], clean[:5])
+    assert torch.isnan(got[5].float()).all()
+
+
+@gpu
+@pytest.mark.parametrize("scale,spread", [(SCALE, 6.0), (1.0, 3.0), (1e-6, 1.0)])
+def test_shared_prefix_mla_wide_scores(scale, spread):
+    """Peaked rows (the running maximum grows late, by much) and flat ones."""
+    q, prefix, tail = prefix_inputs(2, 1, 128, 1030, 40, "cuda", seed=3)
+    prefix *= (torch.linspace(0.01, spread, 1030, device="cuda")[:, None]).bfloat16()
+    out, lse = ops.shared_prefix_mla(q, prefix, tail, None, scale, return_lse=True)
+    check_prefix(q, prefix, tail, None, out, lse, scale)
+
+
+@gpu
+def test_shared_prefix_mla_views_and_streams():
+    g = torch.Generator().manual_seed(4)
+    big = torch.randn(900, 640, generator=g).bfloat16().cuda()
+    prefix = big[10:410:2, 64:]                       # every other row, rows 640 apart
+    buf = torch.randn(40, 3, 576, generator=g).bfloat16().cuda()
+    tail = buf.transpose(0, 1)                        # batch inner, rows strided
+    q = (torch.randn(128, 3, 576, generator=g) * 0.5).bfloat16().cuda().transpose(0, 1)
+    lens = torch.tensor([40, 7, 0], dtype=torch.int32, device="cuda")
+    out = ops.shared_prefix_mla(q, prefix, tail, lens, SCALE)
+    check_prefix(q, prefix, tail, lens.tolist(), out, None)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        other = ops.shared_prefix_mla(q, prefix, tail, lens, SCALE)
+    s.synchronize()
+    assert torch.equal(other, out)
+
+
+@gpu
+def test_shared_prefix_mla_graph_follows_the_lengths():
+    """Captured once, replayed while the tails grow (the lengths are read on the device)."""
+    q, prefix, tail = prefix_inputs(4, 1, 128, 500, 130, "cuda", seed=5)
+    lens = torch.tensor([1, 1, 1, 1], dtype=torch.int32, device="cuda")
+    ops.shared_prefix_mla(q, prefix, tail, lens, SCALE)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = ops.shared_prefix_mla(q, prefix, tail, lens, SCALE, return_lse=True)
+    for now in ([1, 1, 1, 1], [64, 65, 0, 130], [130, 129, 128, 127]):
+        lens.copy_(torch.tensor(now, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        check_prefix(q, prefix, tail, now, out, lse)
+
+
+@gpu
+def test_shared_prefix_mla_bad_length_is_reported():
+    q, prefix, tail = prefix_inputs(2, 1, 128, 10, 4, "cuda", seed=6)
+    lens = torch.tensor([5, -1], dtype=torch.int32, device="cuda")
+    out = ops.shared_prefix_mla(q, prefix, tail, lens, SCALE)
+    with pytest.raises(ops.native.DeviceError):
+        ops.check_errors("cuda")
+    check_prefix(q, prefix, tail, [4, 0], out, None)  # clamped
+
+
+@gpu
+def test_shared_prefix_mla_matches_sparse_mla():
+    """With every record selected the sparse kernel attends to the same set."""
+    q, prefix, tail = prefix_inputs(2, 1, 128, 300, 20, "cuda", seed=7)
+    out = ops.shared_prefix_mla(q[:, 0], prefix, tail, None, SCALE)
+    for b in range(2):
+        kv = torch.cat((prefix, tail[b])).contiguous()
+        ids = torch.arange(320, dtype=torch.int32, device="cuda")[None]
+        want = ops.sparse_mla(q[b], kv, ids, SCALE)
+        # Two kernels with one rounding of P and of the output each.
+        _, _, mag, _ = prefix_oracle(q[b:b + 1, 0], prefix, tail[b:b + 1], [20], SCALE, 512)
+        assert ((out[b].double() - want[0].double()).abs() <= 2.0**-7 * mag[0] + 2.0**-18).all()
+
+
+@pytest.mark.parametrize("T", [1, 3])
+def test_shared_prefix_mla_cpu(T):
+    q, prefix, tail = prefix_inputs(3, T, 4, 50, 6, "cpu", D=80)
+    lens = torch.tensor([6, 0, 2], dtype=torch.int32)
+    out, lse = ops.shared_prefix_mla(q, prefix, tail, lens, 0.2, return_lse=True, value_dim=64)
+    check_prefix(q, prefix, tail, lens.tolist(), out, lse, 0.2)
+    none = ops.shared_prefix_mla(q, prefix[:0], tail, torch.zeros(3, dtype=torch.int32), 0.2, value_dim=64)
+    assert not none.float().abs().any()
+
+
+def test_shared_prefix_mla_refusals():
+    q, prefix, tail = prefix_inputs(2, 1, 4, 8, 3, "cpu", D=80)
+    lens = torch.tensor([1, 2], dtype=torch.int32)
+    for bad in (lambda: ops.shared_prefix_mla(q[0, 0], prefix, tail, lens, 1.0),
+                lambda: ops.shared_prefix_mla(q, prefix[:, :64], tail, lens, 1.0),
+                lambda: ops.shared_prefix_mla(q, prefix, tail[:1], lens, 1.0),
+                lambda: ops.shared_prefix_mla(q, prefix, tail, lens[:1], 1.0),
+                lambda: ops.shared_prefix_mla(q, prefix, None, lens, 1.0),
+                lambda: ops.shared_prefix_mla(q, prefix, tail, lens, 0.0),
+                lambda: ops.shared_prefix_mla(q, prefix, tail, lens, math.inf)):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(IndexError):
+        ops.shared_prefix_mla(q, prefix, tail, torch.tensor([4, 0], dtype=torch.int32), 1.0, value_dim=64)
+
+
+@gpu
+def test_shared_prefix_mla_gpu_refusals():
+    q, prefix, tail = prefix_inputs(2, 1, 128, 8, 3, "cuda")
+    lens = torch.tensor([1, 2], dtype=torch.int32, device="cuda")
+    for bad in (lambda: ops.shared_prefix_mla(q.float(), prefix, tail, lens, 1.0),
+                lambda: ops.shared_prefix_mla(q, prefix.half(), tail, lens, 1.0),
+                lambda: ops.shared_prefix_mla(q, prefix, tail, lens.long(), 1.0),
+                lambda: ops.shared_prefix_mla(q, prefix, tail, lens.cpu(), 1.0),
+                lambda: ops.shared_prefix_mla(q[..., :512], prefix[:, :512], tail[..., :512], lens, 1.0),
+                lambda: ops.shared_prefix_mla(q, torch.zeros(8, 580, device="cuda").bfloat16()[:, 1:577], tail, lens, 1.0),
+                lambda: ops.shared_prefix_mla(q, torch.zeros(576, 8, device="cuda").bfloat16().t(), tail, lens, 1.0)):
+        with pytest.raises(ValueError):
+            bad()
+
+
+# ---------------------------------------------------------------- sampling
+FIXED = 2.0**36
+
+
+def sample_oracle(x, u, T, k, p, mp):
+    """(token, lowest and highest log-probability, margin): the rule in float64.  margin is the relative distance
+    of the draw and of the min-p cut from changing; a top-p cut within 2^-17 of its neighbours is taken both ways."""
+    x = torch.where(torch.isnan(x.double()), -math.inf, x.double())
+    ranked, order = torch.sort(x, descending=True, stable=True)
+    if ranked[0] == -math.inf:
+        return -1, -math.inf, -math.inf, 1.0
+    if not T > 0:
+        return int(order[0]), 0.0, 0.0, 1.0
+    d = torch.where(ranked == ranked[0], 0.0, (ranked - ranked[0]) / T)
+    w = torch.where(ranked == -math.inf, 0.0, torch.exp(d))
+    mass = torch.floor(w * FIXED)
+    V, margin = x.numel(), 1.0
+    n = V if k <= 0 else min(k, V)
+    cuts = [n]
+    if p < 1:
+        all_k = mass[:n].sum()
+        before = mass[:n].cumsum(0) - mass[:n]
+        cuts = [max(1, int((before < (p + e if p > 0 else 0.0) * all_k).sum())) for e in (-2.0**-17, 2.0**-17)]
+    if mp == mp and mp > 0:
+        rest = w[ranked < ranked[0]]  # the best tokens' weight is 1 whatever the arithmetic
+        if rest.numel():
+            margin = min(margin, float((rest / mp - 1).abs().min()))
+        cuts = [max(1, min(n, int((w >= mp).sum()))) for n in cuts]
+    found = []
+    for n in cuts:
+        ids, by = torch.sort(order[:n])
+        cum = mass[:n][by].cumsum(0)
+        target = min(math.floor(u * float(cum[-1])), float(cum[-1]) - 1)
+        if n > 1:
+            margin = min(margin, float((cum / cum[-1] - u).abs().min()))
+        j = int((cum <= target).sum())
+        found.append((int(ids[j]), float(d[by[j]] - torch.log(cum[-1] / FIXED))))
+    if found[0][0] != found[-1][0]:
+        margin = 0.0
+    return found[0][0], found[-1][1], found[0][1], margin
+
+
+def check_sample(logits, u, tokens, logprobs, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, least=0.9):
+    """Rows whose draw is further than 2^-17 from changing (FP32 weights are within ~2^-20) must agree."""
+    R = logits.shape[0]
+    sure = 0
+
+    def at(v, r):
+        return float(v[r]) if torch.is_tensor(v) else float(torch.tensor(v, dtype=torch.float32))
+
+    x = logits.detach().cpu()
+    for r in range(R):
+        tok, low, high, margin = sample_oracle(x[r], float(u[r]), at(temperature, r), int(at(top_k, r)),
+                                               at(top_p, r), at(min_p, r))
+        if margin < 2.0**-17:
+            continue
+        sure += 1
+        assert int(tokens[r]) == tok, f"row {r}"
+        if math.isinf(low):
+            assert float(logprobs[r]) == low
+        else:
+            # (x - max) / T in FP32 is within 2^-23 of itself, the sum of weights within 2^-20, the result rounded once.
+            tol = 2.0**-19 + 2.0**-21 * (abs(low) + 30)
+            assert low - tol <= float(logprobs[r]) <= high + tol
+    assert sure >= least * R
+
+
+def rows(R, V, seed=0, dtype=torch.float32, device="cuda"):
+    g = torch.Generator().manual_seed(seed)
+    x = (torch.randn(R, V, generator=g) * 2 - torch.log(torch.rand(R, V, generator=g).clamp_min(1e-12))).to(dtype)
+    return x.to(device), torch.rand(R, generator=g).to(device)
+
+
+DEVICES = ["cpu", pytest.param("cuda", marks=gpu)]
+SETTINGS = [
+    dict(),
+    dict(temperature=0.0),
+    dict(temperature=0.3),
+    dict(temperature=8.0),
+    dict(top_k=1),
+    dict(top_k=7),
+    dict(top_k=10**9),
+    dict(top_p=0.0),
+    dict(top_p=0.5),
+    dict(top_p=0.999),
+    dict(min_p=0.1),
+    dict(min_p=1.0),
+    dict(temperature=0.7, top_k=50, top_p=0.9, min_p=0.02),
+    dict(temperature=3.0, top_k=900, top_p=0.95),
+]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("params", SETTINGS, ids=str)
+@pytest.mark.parametrize("V", [1, 2, 33, 1024, 5003])
+def test_sample_settings(device, params, V):
+    x, u = rows(6, V, seed=V, device=device)
+    tok, lp = ops.sample_tokens(x, u, **params)
+    check_sample(x, u, tok, lp, **params, least=0.5)
+
+
+@gpu
+@pytest.mark.parametrize("V", [31999, 129280, 200003])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_sample_large_vocabularies(V, dtype):
+    x, u = rows(12, V, seed=1, dtype=dtype)
+    i = torch.arange(12, device="cuda")
+    params = dict(temperature=torch.tensor([0.0, 0.6, 1.0, 2.5], device="cuda")[i % 4],
+                  top_k=torch.tensor([0, 40, 3000], dtype=torch.int32, device="cuda")[i % 3],
+                  top_p=torch.tensor([1.0, 0.9, 0.3], device="cuda")[(i // 3) % 3],
+                  min_p=torch.tensor([0.0, 0.001], device="cuda")[i % 2])
+    tok, lp = ops.sample_tokens(x, u, **params)
+    check_sample(x, u, tok, lp, **params, least=0.7)
+
+
+@gpu
+def test_sample_many_rows_and_batch_independence():
+    """A row's draw does not depend on the batch around it (few rows and many take different splits)."""
+    x, u = rows(300, 4099, seed=2)
+    tok, lp = ops.sample_tokens(x, u, temperature=0.9, top_p=0.95)
+    check_sample(x, u, tok, lp, temperature=0.9, top_p=0.95)
+    for r in (0, 7, 299):
+        t1, l1 = ops.sample_tokens(x[r:r + 1], u[r:r + 1], temperature=0.9, top_p=0.95)
+        assert int(t1) == int(tok[r]) and float(l1) == float(lp[r])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_sample_masked_and_odd_values(device):
+    inf, nan = math.inf, math.nan
+    V = 70
+    x = torch.zeros(9, V)
+    x[0] = -inf                                   # nothing to draw
+    x[1] = nan
+    x[2] = -inf
+    x[2, 41] = 3.0                                # one token left
+    x[3, ::2] = nan                               # every other token masked
+    x[4] = 5.0                                    # all equal
+    x[5, 10] = inf
+    x[5, 60] = inf                                # only infinite ones can be drawn
+    x[6] = torch.finfo(torch.float32).min         # the type's lowest value is a value, not a mask
+    x[6, 3] = 0.0
+    x[7] = torch.finfo(torch.float32).min
+    x[8, :35] = -0.0                              # -0 equals +0
+    u = torch.tensor([0.3, 0.3, 0.3, 0.6, 0.5, 0.75, 0.99, 0.5, 0.25])
+    x, u = x.to(device), u.to(device)
+    tok, lp = ops.sample_tokens(x, u)
+    assert tok.tolist() == [-1, -1, 41, 43, 35, 60, 3, 35, 17]
+    want = [-inf, -inf, 0.0, -math.log(35), -math.log(70), -math.log(2), 0.0, -math.log(70), -math.log(70)]
+    for a, b in zip(lp.tolist(), want):
+        assert a == b or abs(a - b) < 1e-6
+    tok, _ = ops.sample_tokens(x, u, temperature=0.0)
+    assert tok.tolist() == [-1, -1, 41, 1, 0, 10, 3, 0, 0]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("V", [100, 4096, 20001])
+def test_sample_ties_are_cut_by_index(device, V):
+    """Equal logits: top-k and top-p keep the lowest indices."""
+    x = torch.full((4, V), 1.0, device=device)
+    x[:, V // 2] = 2.0
+    top = torch.full((4,), 1 - 2.0**-24, device=device)
+    tok, _ = ops.sample_tokens(x, top, top_k=11)
+    assert tok.tolist() == [max(9, V // 2 if V // 2 > 9 else 9)] * 4
+    flat = torch.full((3, V), -4.0, device=device)
+    tok, lp = ops.sample_tokens(flat, top[:3], top_p=0.5)
+    assert tok.tolist() == [-(-V // 2) - 1] * 3
+    assert abs(float(lp[0]) + math.log(-(-V // 2))) < 1e-5
+    tok, _ = ops.sample_tokens(flat, top[:3], top_k=V // 3, top_p=0.5)
+    assert tok.tolist() == [-(-(V // 3) // 2) - 1] * 3
+    three = torch.full((2, V), -1.0, device=device)
+    three[:, ::3] = 0.25
+    n = len(range(0, V, 3))
+    tok, _ = ops.sample_tokens(three, top[:2], top_k=n - 1)
+    assert tok.tolist() == [3 * (n - 2)] * 2
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_sample_extreme_draws(device):
+    x, _ = rows(5, 999, seed=3, device=device)
+    u = torch.tensor([0.0, 1 - 2.0**-24, 1.0, 7.0, -3.0], device=device)
+    tok, _ = ops.sample_tokens(x, u, top_p=0.8)  # numbers outside [0, 1) end at the nearest kept token
+    lo, _ = ops.sample_tokens(x, torch.zeros(5, device=device), top_p=0.8)
+    hi, _ = ops.sample_tokens(x, torch.full((5,), 1 - 2.0**-24, device=device), top_p=0.8)
+    assert tok[0] == lo[0] and tok[4] == lo[4] and tok[1] == hi[1] and tok[2] >= hi[2] and tok[3] == tok[3]
+    t, _ = ops.sample_tokens(x, torch.full((5,), math.nan, device=device), top_p=0.8)
+    assert torch.equal(t, lo)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_sample_frequencies(device):
+    """8,192 evenly spaced draws of one row: each kept token's share is its probability to one draw."""
+    n = 8192
+    x = torch.randn(1, 40, generator=torch.Generator().manual_seed(5)).to(device)
+    u = ((torch.arange(n) + 0.5) / n).to(device)
+    tok, lp = ops.sample_tokens(x.expand(n, 40), u, temperature=0.8, top_k=12)
+    w = torch.softmax(x[0].double().cpu() / 0.8, -1)
+    kept = torch.zeros(40, dtype=torch.bool)
+    kept[torch.topk(w, 12).indices] = True
+    w = torch.where(kept, w, 0.0)
+    w /= w.sum()
+    share = torch.bincount(tok.cpu(), minlength=40).double() / n
+    assert ((share - w).abs() <= 1.5 / n).all()
+    assert ((lp.cpu().double() - torch.log(w[tok.cpu()])).abs() < 1e-5).all()
+
+
+@gpu
+def test_sample_strided_rows_streams_and_graph():
+    x, u = rows(8, 6000, seed=6)
+    wide = torch.zeros(8, 7001, device="cuda")
+    wide[:, 3:6003] = x
+    want = ops.sample_tokens(x, u, top_k=100)
+    for a, b in zip(ops.sample_tokens(wide[:, 3:6003], u, top_k=100), want):  # rows off 16-byte boundaries
+        assert torch.equal(a, b)
+    for a, b in zip(ops.sample_tokens(x.t().contiguous().t(), u, top_k=100), want):
+        assert torch.equal(a, b)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = ops.sample_tokens(x, u, top_k=100)
+    s.synchronize()
+    assert torch.equal(got[0], want[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gt, gl = ops.sample_tokens(x, u, top_k=100)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(gt, want[0]) and torch.equal(gl, want[1])
+
+
+def test_sample_refusals():
+    x, u = rows(3, 10, device="cpu")
+    for bad in (dict(temperature=-1.0), dict(temperature=math.nan), dict(temperature=math.inf), dict(top_k=-1),
+                dict(top_k=1.5), dict(top_p=-0.1), dict(top_p=1.1), dict(min_p=2.0),
+                dict(temperature=torch.ones(2)), dict(top_k=torch.ones(3)), dict(top_p=torch.ones(3).double())):
+        with pytest.raises(ValueError):
+            ops.sample_tokens(x, u, **bad)
+    for args in ((x[0], u), (x, u[:2]), (x, u.double()), (x.half(), u), (x[:, :0], u)):
+        with pytest.raises(ValueError):
+            ops.sample_tokens(*args)
+    tok, lp = ops.sample_tokens(x[:0], u[:0])
+    assert tok.shape == (0,) and lp.shape == (0,)
+    assert ref.SAMPLE_FIXED == FIXED
