@@ -51,12 +51,12 @@ def check_prefix(q, prefix, tail, lens, got, lse, scale=SCALE):
     dv = got.shape[-1]
     full = lens if lens is not None or tail is None else [tail.shape[1]] * q.shape[0]
     want, wlse, mag, size = prefix_oracle(q, prefix, tail, full, scale, dv)
-    # The probabilities and the output are rounded to BF16 once each (2^-9 relative): |error| <=
-    # 2^-9 sum p|v| + 2^-9 |out| <= 2^-8 sum p|v|.  The scores are FP32 sums of 576 exact products, each
+    # The probabilities and the output are rounded to BF16 once each: 8 significant bits, so half a unit in
+    # the last place is up to 2^-8 relative, and |error| <= 2^-8 sum p|v| + 2^-8 |out| <= 2^-7 sum p|v|.  The scores are FP32 sums of 576 exact products, each
     # step within 2^-23 of the running sum (a random walk of ~sqrt(576) steps is taken as 32): their error
     # adds twice that (numerator and denominator) relative to the same sum.
     score_err = 32 * 2.0**-23 * size
-    bound = (2.0**-8 + 2 * score_err[..., None] + 2.0**-20) * mag + 1e-30
+    bound = (2.0**-7 + 2 * score_err[..., None] + 2.0**-16) * mag + 1e-30
     err = (got.double() - want).abs()
     assert torch.isfinite(got).all()
     assert (err <= bound).all(), f"output off by {(err / bound).max().item():.2f} of its bound"
@@ -200,9 +200,9 @@ def test_shared_prefix_mla_matches_sparse_mla():
         kv = torch.cat((prefix, tail[b])).contiguous()
         ids = torch.arange(320, dtype=torch.int32, device="cuda")[None]
         want = ops.sparse_mla(q[b], kv, ids, SCALE)
-        # Two kernels with one rounding of P and of the output each.
+        # Two kernels with one rounding of P and of the output each, up to 2^-7 sum p|v| apiece.
         _, _, mag, _ = prefix_oracle(q[b:b + 1, 0], prefix, tail[b:b + 1], [20], SCALE, 512)
-        assert ((out[b].double() - want[0].double()).abs() <= 2.0**-7 * mag[0] + 2.0**-18).all()
+        assert ((out[b].double() - want[0].double()).abs() <= 2.0**-6 * mag[0] + 2.0**-18).all()
 
 
 @pytest.mark.parametrize("T", [1, 3])
