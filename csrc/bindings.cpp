@@ -446,7 +446,10 @@ void shared_prefix_mla(const Tensor& q, const Tensor& prefix, const c10::optiona
     TORCH_CHECK(lse->is_contiguous() && lse->numel() == q.size(0) * q.size(1) * q.size(2), "shared_prefix_mla: lse");
     a.lse = ptr<float>(*lse);
   }
-  b200::launch_shared_prefix_mla(a, stream());
+  Tensor scratch;
+  const size_t floats = b200::shared_prefix_mla_scratch_floats(a);
+  if (floats) scratch = torch::empty({int64_t(floats)}, torch::dtype(torch::kFloat32).device(q.device()));
+  b200::launch_shared_prefix_mla(a, floats ? scratch.data_ptr<float>() : nullptr, stream());
 }
 
 void sample_tokens(const Tensor& logits, const Tensor& u, const c10::optional<Tensor>& temperature,

@@ -22,7 +22,9 @@ struct PrefixMLAArgs {
   float scale;
   int* err;
 };
-void launch_shared_prefix_mla(const PrefixMLAArgs& a, cudaStream_t stream);
+// FP32 workspace of a call (0: none); the same arguments give the same plan.
+size_t shared_prefix_mla_scratch_floats(const PrefixMLAArgs& a);
+void launch_shared_prefix_mla(const PrefixMLAArgs& a, float* scratch, cudaStream_t stream);
 
 // ---------------------------------------------------------------- sampling
 struct SampleArgs {

@@ -5,8 +5,47 @@
 //   out  = sum_j exp(s(j) - m) v_j / sum_j exp(s(j) - m),  m = max_j s(j),
 //   lse  = m + log sum_j exp(s(j) - m),  v_j = the first 512 dims of k_j.
 //
-// One warp per (query, head) walks the keys once with a running maximum and
-// sum (FP32); each lane holds 18 query dims and 16 output dims.
+// Every (query, head) row attends to the same prefix, so the B * T * H rows are
+// cut into tiles of 128 rows whatever head or continuation they belong to, and
+// a tile is a dense product with the prefix: S = Q K^T, O += P V on the tensor
+// cores, P = exp2(S - m) in between (one pass over the keys with a running
+// maximum and sum).  With B * T * H rows an HBM byte of the prefix feeds
+// 2 * 1088 / 1152 * rows operations, so from about 140 rows on the tensor cores
+// are the bound, not HBM; the prefix is re-read per row tile from L2.
+//
+// A unit of work is (row tile, range of 64-key tiles), run by a pair of SMs
+// (tcgen05 cta_group::2, M = 128):
+//  * CTA c holds Q rows [64c, +64) in shared memory, and in TMEM the S and O
+//    accumulators of those rows (a 64 x N accumulator takes N / 2 columns, so O
+//    takes 256 columns and stays on chip next to four S buffers).
+//  * QK (N = 64): CTA c supplies the full records of keys [32c, +32) of a tile.
+//  * PV (two MMAs of N = 256 value dims): CTA c supplies dims [256v + 128c, +128)
+//    of all 64 keys.  Its own keys' dims are already there; the peer keys' dims
+//    are loaded, once QK is done with the tile, over record chunks of its own
+//    keys that only QK needed, at the offsets where the peer holds them (so one
+//    descriptor serves both CTAs): 52 KB per tile and CTA instead of 68 KB.
+//  * Records are dense rows, so a tile is nine TMA loads of 32 rows x 64 dims
+//    (128-byte swizzle) and four more for the peer keys' dims, all issued by one
+//    thread and completing on CTA 0's barriers.  Tail tiles are loaded by
+//    cp.async instead, which zero-fills the rows past the visible ones: memory
+//    there may hold NaN, and 0 * NaN in PV would spread it.
+//  * Softmax: 8 warps; the four threads of a row (TMEM lanes r and r + 64, two
+//    warpgroups) take 16 keys of a tile each and agree on the maximum through
+//    shared memory.  The running maximum is raised only when it grows by more
+//    than 2^8 (O is then rescaled), P is rounded to BF16 (what the MMA takes),
+//    its sum is kept unrounded in FP32.
+//
+// Row tiles rarely fill the SM pairs evenly, so the key ranges of the tiles
+// that do not make up whole waves are cut into equal shares, one per pair; a
+// tile that falls into several shares leaves FP32 partials that a second kernel
+// merges by their LSE.  When a row tile holds rows of several continuations (H
+// not a multiple of 128), tails are units of their own (one per query) and the
+// same kernel merges them.
+//
+// All waits are bounded (error word, then the CTA drains and exits).
+#include <algorithm>
+#include <vector>
+
 #include "../common/host.h"
 #include "../common/ptx.cuh"
 #include "generation.h"
@@ -16,82 +55,766 @@ namespace {
 
 constexpr int D = 576;
 constexpr int DV = 512;
-constexpr int kWarps = 8;
+constexpr int BM = 128;                   // rows per unit (pair)
+constexpr int MC = 64;                    // rows per CTA
+constexpr int BN = 64;                    // keys per tile (pair)
+constexpr int BNC = 32;                   // keys per tile per CTA (QK's B split)
+constexpr int STAGES = 3;                 // record ring (a stage is held from its load to the tile's PV)
+constexpr int SBUF = 4;                   // S buffers in TMEM
+constexpr int kChunks = D / 64;
+constexpr int kQChunkBytes = MC * 128;
+constexpr int kKeyChunkBytes = BNC * 128;
+constexpr int kPBytes = MC * 128;         // 64 rows x 64 keys BF16
+constexpr int kSoftmaxWarps = 8;          // warps 0-7
+constexpr int kSoftmaxThreads = kSoftmaxWarps * 32;
+constexpr int kOwnWarp0 = 8;              // warps 8, 9: Q + records
+constexpr int kOwnWarps = 2;
+constexpr int kPvWarp0 = 10;              // warps 10, 11: peer keys' value dims
+constexpr int kPvWarps = 2;
+constexpr int kMmaWarp = 12;
+constexpr int kThreads = 13 * 32;
+constexpr uint32_t kQBytes = kChunks * kQChunkBytes;
+constexpr uint32_t kOwnBytes = kChunks * kKeyChunkBytes;  // records of a CTA's 32 keys
+constexpr uint32_t kPvBytes = 4 * kKeyChunkBytes;         // the peer's 32 keys x 256 value dims
+constexpr float kRescaleThreshold = 8.f;                  // log2 units
+constexpr uint32_t kTmemS = 256;                          // O half v at [128v, +128), S buffers at 256 + 32b
 
-__global__ void __launch_bounds__(kWarps * 32) prefix_mla_kernel(PrefixMLAArgs a) {
-  const int lane = threadIdx.x % 32;
-  const int64_t row = int64_t(blockIdx.x) * kWarps + threadIdx.x / 32;
-  const int64_t rows = int64_t(a.B) * a.T * a.H;
-  if (row >= rows) return;
-  const int g = int(row / a.H), b = g / a.T, t = g % a.T;
+constexpr int kOffQ = 0;                                            // [9][8 KB]
+constexpr int kOffOwn = kOffQ + kChunks * kQChunkBytes;             // [STAGES][9][4 KB]
+constexpr int kOffP = kOffOwn + STAGES * kChunks * kKeyChunkBytes;  // [2][8 KB]
+constexpr int kOffSmall = kOffP + 2 * kPBytes;
+
+struct Small {
+  float red[2][kSoftmaxThreads];  // tile maxima of a row's four threads; in the end the denominators
+  uint64_t q_full;                // CTA 0: Q rows of both CTAs
+  uint64_t own_full[STAGES];      // CTA 0: records of the tile
+  uint64_t pv_full[STAGES];       // CTA 0: peer keys' value dims
+  uint64_t pv_done[STAGES];       // PV of the tile done (commit): stage and P buffer free
+  uint64_t s_full[SBUF];          // QK of the tile done (commit)
+  uint64_t s_empty[SBUF];         // CTA 0: both CTAs' softmax warps read S
+  uint64_t p_full[2];             // CTA 0: both CTAs' softmax warps wrote P
+  uint64_t o_full;                // last PV done (commit)
+  uint32_t tmem_base;
+  int abort_flag;
+};
+constexpr size_t kSmemBytes = size_t(kOffSmall) + sizeof(Small);
+static_assert(kSmemBytes <= 232448, "shared_prefix_mla: shared memory over the per-block limit");
+
+// Work list: units [0, full) are whole row tiles; units [full, full + cut) are
+// shares of the remaining tiles; then, when tails are apart, one unit per query
+// and 128 heads.  Slot = index of a unit's FP32 partial, -1: written directly.
+constexpr int kMaxShares = 256;
+struct Share {
+  int tile, t0, t1, slot;
+};
+struct Plan {
+  int full = 0, cut = 0, tails = 0;  // units of each kind
+  int apart = 0;                     // tails are units of their own
+  int tiles = 0;                     // 64-key tiles of a row tile's list (prefix, then the joined tail)
+  int slots = 0;
+  Share share[kMaxShares];
+};
+// Merged row tiles: tile0 + i.  The first `single` have one partial each (slot
+// i), the others slots [begin[i - single], begin[i - single + 1]) (none: written directly).
+struct MergePlan {
+  int tile0, tiles, single, tail_slot0, apart;
+  int begin[kMaxShares + 1];
+};
+
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t* dst_smem, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst_smem)),
+               "r"(ncols)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_relinquish_pair() {
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+
+// D[tmem] (+)= A[smem] * B[smem]^T over the pair: each CTA supplies its M/2
+// rows of A and N/2 rows of B at the same shared-memory offsets.
+__device__ __forceinline__ void mma_pair_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Arrive on the mbarrier at shared::cluster address `bar` once the pair's previously issued MMAs complete.
+__device__ __forceinline__ void commit_pair(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool mbar_test_cluster(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Every thread of the barrier gets the OR of the predicates.
+__device__ __forceinline__ bool bar_red_or(uint32_t id, uint32_t nthreads, bool pred) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.or.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(uint32_t(pred)), "r"(id), "r"(nthreads)
+      : "memory");
+  return r != 0;
+}
+// Tiled load into this CTA's shared memory, counted on the mbarrier at
+// shared::cluster address `bar` (CTA 0 of the pair); no cluster fan-out.
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const void* desc, uint32_t bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+      "l"(desc), "r"(bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_expect_tx_at(uint32_t cluster_bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;" ::"r"(cluster_bar), "r"(bytes) : "memory");
+}
+
+// What a unit works on, the same in both CTAs and every role.
+struct Unit {
+  int row0, nrows;     // first flattened row, valid rows of the 128
+  int p0, np;          // prefix tiles [p0, p0 + np)
+  int t0, nt;          // then tail tiles [t0, t0 + nt) of continuation b
+  int b, seen;         // visible tail rows
+  int slot;
+  __device__ int ntiles() const { return np + nt; }
+};
+
+__device__ __forceinline__ int visible_tail(const PrefixMLAArgs& a, int g) {
+  if (a.S == 0) return 0;
   int len = a.S;
   if (a.tail_lens) {
-    len = a.tail_lens[b];
+    len = a.tail_lens[g / a.T];
     if (len < 0 || len > a.S) {
-      if (lane == 0) record_error(a.err, kErrBadIndex);
+      if (threadIdx.x == 0) record_error(a.err, kErrBadIndex);
       len = min(max(len, 0), a.S);
     }
   }
-  const int seen = max(0, len - (a.T - 1 - t));
-  // Lane l holds dims 2l + 64i, 2l + 64i + 1 (i < 9); i < 8 are the value dims.
-  float qf[18], acc[16];
-#pragma unroll
-  for (int i = 0; i < 9; ++i) {
-    const uint32_t v = *reinterpret_cast<const uint32_t*>(a.q + row * D + 64 * i + 2 * lane);
-    qf[2 * i] = bf16_lo(v) * a.scale;
-    qf[2 * i + 1] = bf16_hi(v) * a.scale;
+  return max(0, len - (a.T - 1 - g % a.T));
+}
+
+__device__ __forceinline__ Unit decode_unit(const PrefixMLAArgs& a, const Plan& plan, int u) {
+  Unit w;
+  w.b = 0;
+  w.seen = w.t0 = w.nt = w.p0 = w.np = 0;
+  const int rows = a.B * a.T * a.H;
+  const int prefix_tiles = (a.P + BN - 1) / BN;
+  if (u >= plan.full + plan.cut) {  // a query's tail
+    const int i = u - plan.full - plan.cut;
+    const int per = (a.H + BM - 1) / BM;
+    const int g = i / per, h0 = (i % per) * BM;
+    w.row0 = g * a.H + h0;
+    w.nrows = min(BM, a.H - h0);
+    w.b = g / a.T;
+    w.seen = visible_tail(a, g);
+    w.nt = (w.seen + BN - 1) / BN;
+    w.slot = a.P > 0 ? plan.slots - plan.tails + i : -1;
+    return w;
   }
-#pragma unroll
-  for (int i = 0; i < 16; ++i) acc[i] = 0.f;
-  // The sum runs over blocks of 32 keys first: 1/32 of the roundings of one long chain.
-  float m = -INFINITY, l = 0.f, block = 0.f;
-  for (int j = 0; j < a.P + seen; ++j) {
-    const __nv_bfloat16* k =
-        j < a.P ? a.prefix + int64_t(j) * a.ld_prefix : a.tail + int64_t(b) * a.ld_batch + int64_t(j - a.P) * a.ld_tail;
-    float kf[18];
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 9; ++i) {
-      const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(k + 64 * i + 2 * lane));
-      kf[2 * i] = bf16_lo(v);
-      kf[2 * i + 1] = bf16_hi(v);
-      s = fmaf(qf[2 * i], kf[2 * i], s);
-      s = fmaf(qf[2 * i + 1], kf[2 * i + 1], s);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (s > m) {
-      const float f = m == -INFINITY ? 0.f : expf(m - s);
-      l *= f;
-      block *= f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) acc[i] *= f;
-      m = s;
-    }
-    const float p = m == -INFINITY ? 0.f : expf(s - m);
-    block += p;
-    if (j % 32 == 31) {
-      l += block;
-      block = 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) acc[i] = fmaf(p, kf[i], acc[i]);
+  int tile = u, k0 = 0, k1 = plan.tiles;
+  w.slot = plan.apart && plan.tails ? u : -1;
+  if (u >= plan.full) {
+    const Share& s = plan.share[u - plan.full];
+    tile = s.tile;
+    k0 = s.t0;
+    k1 = s.t1;
+    w.slot = s.slot;
   }
-  l += block;
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  w.row0 = tile * BM;
+  w.nrows = min(BM, rows - w.row0);
+  w.p0 = min(k0, prefix_tiles);
+  w.np = min(k1, prefix_tiles) - w.p0;
+  if (!plan.apart && k1 > prefix_tiles) {
+    const int g = w.row0 / a.H;
+    w.b = g / a.T;
+    w.seen = visible_tail(a, g);
+    w.t0 = max(k0, prefix_tiles) - prefix_tiles;
+    w.nt = max(0, min(k1 - prefix_tiles, (w.seen + BN - 1) / BN) - w.t0);
+  }
+  return w;
+}
+
+__global__ void __launch_bounds__(kThreads, 1)
+    prefix_mla_kernel(const __grid_constant__ PrefixMLAArgs a, const __grid_constant__ Plan plan,
+                      const __grid_constant__ CUtensorMap tma_q, const __grid_constant__ CUtensorMap tma_kv,
+                      float scale_log2, float* __restrict__ part_o,
+                      float* __restrict__ part_lse) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  pdl_wait();
+  uint8_t* base = smem_raw;
+  const uint32_t sbase = smem_u32(base);
+  if (sbase & 1023u) {  // uniform over the cluster; the swizzle atoms need it and there is no room for slack
+    if (threadIdx.x == 0) record_error(a.err, kErrBadIndex);
+    return;
+  }
+  Small& s = *reinterpret_cast<Small*>(base + kOffSmall);
+  const uint32_t crank = cluster_ctarank();
+  const Unit w = decode_unit(a, plan, int(blockIdx.x >> 1));
+  const int ntiles = w.ntiles();
+  const int warp = threadIdx.x / 32;
+  const int lane = threadIdx.x % 32;
+
+  auto own_chunk = [&](int st, int j) { return sbase + kOffOwn + (st * kChunks + j) * kKeyChunkBytes; };
+  // PV's B operand (value dims, MN-major) of key half kh and value half v.
+  auto pv_region = [&](int st, int kh, int v) { return own_chunk(st, 4 * v + 2 * kh); };
+  const uint32_t p_buf[2] = {sbase + kOffP, sbase + kOffP + kPBytes};
+  // Tile i: first key row of its source (prefix or tail) and how many of its 64 keys are visible.
+  auto tile_key0 = [&](int i) { return (i < w.np ? w.p0 + i : w.t0 + i - w.np) * BN; };
+  auto tile_valid = [&](int i) { return min(BN, (i < w.np ? a.P : w.seen) - tile_key0(i)); };
+
+  if (threadIdx.x == 0) {
+    mbar_init(&s.q_full, 2);
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&s.own_full[i], 2 * kOwnWarps);
+      mbar_init(&s.pv_full[i], 2 * kPvWarps);
+      mbar_init(&s.pv_done[i], 1);
+    }
+    for (int i = 0; i < SBUF; ++i) {
+      mbar_init(&s.s_full[i], 1);
+      mbar_init(&s.s_empty[i], 2 * kSoftmaxWarps);
+    }
+    for (int i = 0; i < 2; ++i) mbar_init(&s.p_full[i], 2 * kSoftmaxWarps);
+    mbar_init(&s.o_full, 1);
+    s.abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc_pair(&s.tmem_base, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // both CTAs' barriers initialised before any remote arrive
+  pdl_trigger();
+  tc_fence_after();
+  const uint32_t tmem = s.tmem_base;
+  volatile int* abort_flag = &s.abort_flag;
+  int* err = a.err;
+  auto leader = [&](uint64_t* bar) { return mapa_shared(smem_u32(bar), 0); };
+  auto arrive_leader = [&](uint64_t* bar) {
+    if (crank == 0) mbar_arrive(bar);
+    else mbar_arrive_remote(mapa_shared(smem_u32(bar), 0));
+  };
+  const uint8_t* tail_rows = reinterpret_cast<const uint8_t*>(a.tail + int64_t(w.b) * a.ld_batch);
+  const int64_t tail_pitch = a.ld_tail * 2;
+
+  if (ntiles == 0) {
+    // nothing visible: straight to the epilogue
+  } else if (warp >= kOwnWarp0 && warp < kOwnWarp0 + kOwnWarps) {
+    // --------------------------------------------- Q rows + QK records
+    const int ow = warp - kOwnWarp0;
+    if (ow == 0 && lane == 0) {
+      mbar_arrive_expect_tx_at(leader(&s.q_full), kQBytes);
+#pragma unroll 1
+      for (int j = 0; j < kChunks; ++j)
+        tma_load_pair(sbase + kOffQ + j * kQChunkBytes, &tma_q, leader(&s.q_full), 64 * j, w.row0 + MC * int(crank));
+    }
+    for (int i = 0; i < ntiles; ++i) {
+      const int st = i % STAGES;
+      if (!__all_sync(0xffffffffu, mbar_wait(&s.pv_done[st], ((i / STAGES) & 1) ^ 1, err, kErrTimeoutSmemEmpty,
+                                             abort_flag)))
+        break;
+      const int key0 = tile_key0(i) + BNC * int(crank);
+      if (i < w.np) {
+        if (lane == 0) {
+          if (ow == 0) {
+            mbar_arrive_expect_tx_at(leader(&s.own_full[st]), kOwnBytes);
+#pragma unroll 1
+            for (int j = 0; j < kChunks; ++j)
+              tma_load_pair(own_chunk(st, j), &tma_kv, leader(&s.own_full[st]), 64 * j, key0);
+          } else {
+            arrive_leader(&s.own_full[st]);
+          }
+        }
+      } else {
+#pragma unroll 4
+        for (int e = ow * 32 + lane; e < BNC * 72; e += kOwnWarps * 32) {
+          const int r = e / 72, u72 = e % 72;
+          const bool ok = key0 + r < w.seen;
+          const uint32_t dst = own_chunk(st, u72 >> 3) + r * 128 + (((u72 & 7) ^ (r & 7)) << 4);
+          cp_async16_zfill(dst, ok ? tail_rows + int64_t(key0 + r) * tail_pitch + u72 * 16 : tail_rows, ok);
+        }
+        cp_async_wait_all();
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) arrive_leader(&s.own_full[st]);
+      }
+      __syncwarp();
+    }
+  } else if (warp >= kPvWarp0 && warp < kPvWarp0 + kPvWarps) {
+    // ------------------------------------------- peer keys' value dims
+    const int pw = warp - kPvWarp0;
+    const int peer = 1 - int(crank);
+    for (int i = 0; i < ntiles; ++i) {
+      const int st = i % STAGES;
+      // QK of the tile is done with the chunks the dims land in.
+      if (!__all_sync(0xffffffffu, mbar_wait(&s.s_full[i % SBUF], (i / SBUF) & 1, err, kErrTimeoutSmemEmpty,
+                                             abort_flag)))
+        break;
+      const int key0 = tile_key0(i) + BNC * peer;
+      if (i < w.np) {
+        if (lane == 0) {
+          if (pw == 0) {
+            mbar_arrive_expect_tx_at(leader(&s.pv_full[st]), kPvBytes);
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    *reinterpret_cast<uint32_t*>(a.out + row * DV + 64 * i + 2 * lane) = pack_bf16(acc[2 * i] * inv, acc[2 * i + 1] * inv);
-  if (a.lse && lane == 0) a.lse[row] = l > 0.f ? m + logf(l) : -INFINITY;
+            for (int c = 0; c < 4; ++c)
+              tma_load_pair(pv_region(st, peer, c >> 1) + (c & 1) * kKeyChunkBytes, &tma_kv, leader(&s.pv_full[st]),
+                            64 * (4 * (c >> 1) + 2 * int(crank) + (c & 1)), key0);
+          } else {
+            arrive_leader(&s.pv_full[st]);
+          }
+        }
+      } else {
+#pragma unroll 4
+        for (int e = pw * 32 + lane; e < BNC * 32; e += kPvWarps * 32) {
+          const int r = e >> 5, v = (e >> 4) & 1, qc = (e >> 3) & 1, u = e & 7;
+          const bool ok = key0 + r < w.seen;
+          const uint32_t dst = pv_region(st, peer, v) + qc * kKeyChunkBytes + r * 128 + ((u ^ (r & 7)) << 4);
+          const int unit = (4 * v + 2 * int(crank) + qc) * 8 + u;
+          cp_async16_zfill(dst, ok ? tail_rows + int64_t(key0 + r) * tail_pitch + unit * 16 : tail_rows, ok);
+        }
+        cp_async_wait_all();
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) arrive_leader(&s.pv_full[st]);
+      }
+      __syncwarp();
+    }
+  } else if (warp == kMmaWarp) {
+    if (crank == 0 && elect_one()) {
+      // ------------------------------------------------------- MMA issuer
+      const uint32_t idesc_qk = umma_idesc(128, BN, 1, 1);
+      const uint32_t idesc_pv = umma_idesc(128, 256, 1, 1) | (1u << 16);  // B (V) MN-major
+      auto peer = [&](uint64_t* bar) { return mapa_shared(smem_u32(bar), 1); };
+      bool ok = mbar_wait_cluster(&s.q_full, 0, err, kErrTimeoutTmaFull, abort_flag);
+      auto issue_qk = [&](int i) {
+        const int st = i % STAGES, b = i % SBUF;
+        fence_proxy_async();  // cp.async rows (generic proxy) before the tensor core reads them
+        tc_fence_after();
+        const uint32_t d = tmem + kTmemS + b * (BN / 2);
+#pragma unroll 1
+        for (int j = 0; j < kChunks; ++j) {
+          const uint64_t adesc = umma_desc_sw128(sbase + kOffQ + j * kQChunkBytes);
+          const uint64_t bdesc = umma_desc_sw128(own_chunk(st, j));
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            mma_pair_ss(d, adesc + ((k * 32) >> 4), bdesc + ((k * 32) >> 4), idesc_qk, (j > 0 || k > 0) ? 1u : 0u);
+        }
+        commit_pair(smem_u32(&s.s_full[b]));
+        commit_pair(peer(&s.s_full[b]));
+      };
+      auto issue_pv = [&](int i) {
+        const int st = i % STAGES, b = i & 1;
+        fence_proxy_async();
+        tc_fence_after();
+        const uint64_t pdesc = umma_desc_sw128(p_buf[b]);
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            // Keys [16k, +16): key half k / 2, row offset 16 (k % 2) in its region.
+            const uint64_t vdesc = umma_desc_sw128_mn(pv_region(st, k >> 1, v) + (k & 1) * 16 * 128, kKeyChunkBytes);
+            mma_pair_ss(tmem + v * 128, pdesc + ((k * 32) >> 4), vdesc, idesc_pv, (i > 0 || k > 0) ? 1u : 0u);
+          }
+        }
+        commit_pair(smem_u32(&s.pv_done[st]));
+        commit_pair(peer(&s.pv_done[st]));
+      };
+      int nq = 0, np = 0;
+      uint64_t idle_since = 0;
+      while (ok && np < ntiles) {
+        bool progressed = false;
+        if (nq < ntiles && mbar_test_cluster(&s.own_full[nq % STAGES], (nq / STAGES) & 1) &&
+            mbar_test_cluster(&s.s_empty[nq % SBUF], ((nq / SBUF) & 1) ^ 1)) {
+          issue_qk(nq++);
+          progressed = true;
+        }
+        if (np < nq && mbar_test_cluster(&s.p_full[np & 1], (np >> 1) & 1) &&
+            mbar_test_cluster(&s.pv_full[np % STAGES], (np / STAGES) & 1)) {
+          issue_pv(np++);
+          progressed = true;
+        }
+        if (progressed) {
+          idle_since = 0;
+        } else if (idle_since == 0) {
+          idle_since = globaltimer_ns();
+        } else if (globaltimer_ns() - idle_since > kWaitBudgetNs || *abort_flag) {
+          record_error(err, kErrTimeoutGeneric);
+          *abort_flag = 1;
+          ok = false;
+        }
+      }
+      if (ok) {
+        commit_pair(smem_u32(&s.o_full));
+        commit_pair(peer(&s.o_full));
+      }
+    }
+  }
+
+  if (warp < kSoftmaxWarps) {
+    // ------------------------------------------------------------ softmax
+    // The threads leave the tile loop together: a failed wait is carried to
+    // the next bar.red.or, which every thread reaches.  TMEM loads and stores
+    // run only under warp-uniform conditions.
+    const int tt = threadIdx.x;
+    const int wg = tt >> 7;             // warpgroup: which 16 of the lane's 32 S columns
+    const int hrow = tt & 63;           // row within the CTA
+    const int kh = (tt >> 6) & 1;       // key half (CTA kh's keys)
+    const uint32_t lane_addr = uint32_t((warp & 3) * 32) << 16;
+    const int col0 = 32 * kh + 16 * wg; // first key of this thread in a tile
+    float m_used = -INFINITY, l = 0.f;
+    bool pending_fail = false;
+    bool failed = false;
+    for (int i = 0; i < ntiles; ++i) {
+      const int b = i % SBUF;
+      const int pb = i & 1;
+      const int valid = tile_valid(i) - col0;  // this thread's keys j < valid count
+      bool got = __all_sync(0xffffffffu, mbar_wait(&s.s_full[b], (i / SBUF) & 1, err, kErrTimeoutTmemFull, abort_flag));
+      uint32_t r[16];
+      if (got) {
+        tc_fence_after();
+        tmem_ld16(tmem + lane_addr + kTmemS + b * (BN / 2) + 16 * wg, r);
+        tmem_wait_ld();
+        tmem_regs_ready16(r);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_leader(&s.s_empty[b]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) r[j] = 0u;
+      }
+      if (valid < 16) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (j >= valid) r[j] = 0xff800000u;  // -inf: weight 0
+      }
+      float mx[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        mx[j] = fmaxf(fmaxf(__uint_as_float(r[j]), __uint_as_float(r[j + 4])),
+                      fmaxf(__uint_as_float(r[j + 8]), __uint_as_float(r[j + 12])));
+      float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2;  // the scale is positive
+      s.red[pb][tt] = mt;
+      if (bar_red_or(1, kSoftmaxThreads, !got || pending_fail)) {
+        failed = true;
+        break;
+      }
+      mt = fmaxf(fmaxf(mt, s.red[pb][tt ^ 64]), fmaxf(s.red[pb][tt ^ 128], s.red[pb][tt ^ 192]));
+      bool rescale = false;
+      float alpha = 1.f;
+      if (m_used == -INFINITY) {
+        m_used = mt;
+      } else if (mt > m_used + kRescaleThreshold) {
+        alpha = exp2f(m_used - mt);
+        l *= alpha;
+        m_used = mt;
+        rescale = true;
+      }
+      const float mbase = m_used == -INFINITY ? 0.f : m_used;
+      uint32_t pk[8];
+      float ps[2] = {0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float x = ex2_approx(fmaf(__uint_as_float(r[2 * j]), scale_log2, -mbase));
+        const float y = ex2_approx(fmaf(__uint_as_float(r[2 * j + 1]), scale_log2, -mbase));
+        ps[j & 1] += x + y;
+        pk[j] = pack_bf16(x, y);
+      }
+      l += ps[0] + ps[1];
+      // P(i) reuses the buffer of P(i - 2): wait for PV(i - 2).
+      bool clear = true;
+      if (i >= 2)
+        clear = __all_sync(0xffffffffu, mbar_wait(&s.pv_done[(i - 2) % STAGES], ((i - 2) / STAGES) & 1, err,
+                                                  kErrTimeoutTmemEmpty, abort_flag));
+      if (clear && i >= 1 && __any_sync(0xffffffffu, rescale)) {
+        // O is touched only after PV(i - 1), the last MMA adding into it, is done.
+        clear = __all_sync(0xffffffffu, mbar_wait(&s.pv_done[(i - 1) % STAGES], ((i - 1) / STAGES) & 1, err,
+                                                  kErrTimeoutTmemEmpty, abort_flag));
+        if (clear) {
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t o[32];
+            tmem_ld32(tmem + lane_addr + wg * 128 + c * 32, o);
+            tmem_wait_ld();
+            tmem_regs_ready(o);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+            tmem_st32(tmem + lane_addr + wg * 128 + c * 32, o);
+          }
+          tmem_wait_st();
+        }
+      }
+      if (!clear) {
+        pending_fail = true;
+        continue;
+      }
+      // P row hrow, keys [col0, +16): two 16-byte units of the swizzled 128-byte row.
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int u = (col0 >> 3) + j;
+        const uint32_t dst = p_buf[pb] + hrow * 128 + ((u ^ (hrow & 7)) << 4);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(pk[4 * j]), "r"(pk[4 * j + 1]),
+                     "r"(pk[4 * j + 2]), "r"(pk[4 * j + 3])
+                     : "memory");
+      }
+      fence_proxy_async();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_leader(&s.p_full[pb]);
+    }
+    // ---- epilogue: O / l over the four threads of each row.  Every read of
+    // red[ntiles & 1] (tile ntiles - 2) happened before the last tile's
+    // barrier, so the buffer is free for the denominators.
+    float* lsum = s.red[ntiles & 1];
+    lsum[tt] = l;
+    const bool any_fail = bar_red_or(1, kSoftmaxThreads, failed || pending_fail);
+    const float lt = (l + lsum[tt ^ 64]) + (lsum[tt ^ 128] + lsum[tt ^ 192]);
+    // A row without visible keys has sum 0; NaN scores stay NaN.
+    const float inv = lt == 0.f ? 0.f : 1.f / lt;
+    const float lse = lt == 0.f ? -INFINITY : (m_used == -INFINITY ? 0.f : m_used) * 0.69314718055994531f + logf(lt);
+    const bool have_o = !any_fail && ntiles > 0 &&
+                        __all_sync(0xffffffffu, mbar_wait(&s.o_full, 0, err, kErrTimeoutTmemFull, abort_flag));
+    if (have_o) tc_fence_after();
+    const int trow = MC * int(crank) + hrow;  // row within the tile
+    const int64_t row = w.row0 + trow;
+    const bool store = trow < w.nrows;
+    // Warpgroup wg owns value half wg: columns [128 wg, +128) = dims 256 wg + 128 kh + [0, 128).
+    if (w.slot < 0 || have_o) {
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        uint32_t r[32];
+        if (have_o) {
+          tmem_ld32(tmem + lane_addr + wg * 128 + c * 32, r);
+          tmem_wait_ld();
+          tmem_regs_ready(r);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) r[j] = 0u;
+        }
+        const int dim0 = 256 * wg + 128 * kh + 32 * c;
+        if (w.slot >= 0) {
+          // [slot][dim][row]: a warp's store is one 128-byte line.
+          float* o = part_o + (int64_t(w.slot) * DV + dim0) * BM + trow;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) o[j * BM] = __uint_as_float(r[j]) * inv;
+        } else if (store) {
+          __nv_bfloat16* o = a.out + row * DV + dim0;
+#pragma unroll
+          for (int j = 0; j < 32; j += 8) {
+            uint4 v;
+            v.x = pack_bf16(__uint_as_float(r[j]) * inv, __uint_as_float(r[j + 1]) * inv);
+            v.y = pack_bf16(__uint_as_float(r[j + 2]) * inv, __uint_as_float(r[j + 3]) * inv);
+            v.z = pack_bf16(__uint_as_float(r[j + 4]) * inv, __uint_as_float(r[j + 5]) * inv);
+            v.w = pack_bf16(__uint_as_float(r[j + 6]) * inv, __uint_as_float(r[j + 7]) * inv);
+            *reinterpret_cast<uint4*>(o + j) = v;
+          }
+        }
+      }
+    }
+    if (wg == 0 && kh == 0) {
+      if (w.slot >= 0) part_lse[int64_t(w.slot) * BM + trow] = have_o ? lse : -INFINITY;
+      else if (a.lse && store) a.lse[row] = lse;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {  // a copy may still be in flight: let it land before the memory is released
+    const uint64_t start = globaltimer_ns();
+    while (globaltimer_ns() - start < 1000000ull) {
+    }
+  }
+  cluster_sync_all();  // no CTA leaves while its peer may still arrive on its barriers
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+// out[row] = sum_s exp(lse_s - lse) o_s over the partials of the row's tile
+// (and of its query's tail).  Thread = row, blockIdx.y = 8 value dims.
+__global__ void __launch_bounds__(BM) prefix_mla_merge_kernel(const __grid_constant__ PrefixMLAArgs a,
+                                                              const __grid_constant__ MergePlan mp,
+                                                              const float* __restrict__ part_o,
+                                                              const float* __restrict__ part_lse) {
+  pdl_trigger();
+  pdl_wait();
+  const int i = blockIdx.x, d0 = blockIdx.y * 8, lane = threadIdx.x;
+  const int64_t row = int64_t(mp.tile0 + i) * BM + lane;
+  if (row >= int64_t(a.B) * a.T * a.H) return;
+  int s0 = i, s1 = i + 1;
+  if (i >= mp.single) {
+    s0 = mp.begin[i - mp.single];
+    s1 = mp.begin[i - mp.single + 1];
+    if (s0 == s1) return;
+  }
+  int64_t tail_slot = -1;
+  int tail_lane = 0;
+  if (mp.apart) {
+    const int g = int(row / a.H), h = int(row % a.H);
+    tail_slot = mp.tail_slot0 + int64_t(g) * ((a.H + BM - 1) / BM) + h / BM;
+    tail_lane = h % BM;
+  }
+  float mx = -INFINITY;
+  for (int s = s0; s < s1; ++s) mx = fmaxf(mx, part_lse[int64_t(s) * BM + lane]);
+  if (tail_slot >= 0) mx = fmaxf(mx, part_lse[tail_slot * BM + tail_lane]);
+  const float base = mx == -INFINITY ? 0.f : mx;
+  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  float wsum = 0.f;
+  auto add = [&](int64_t slot, int l) {
+    const float lse = part_lse[slot * BM + l];
+    if (lse == -INFINITY) return;  // nothing visible there: its partial was not written
+    const float wt = expf(lse - base);
+    wsum += wt;
+    const float* p = part_o + (slot * DV + d0) * BM + l;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] = fmaf(wt, p[j * BM], acc[j]);
+  };
+#pragma unroll 4
+  for (int s = s0; s < s1; ++s) add(s, lane);
+  if (tail_slot >= 0) add(tail_slot, tail_lane);
+  const float inv = wsum == 0.f ? 0.f : 1.f / wsum;
+  uint4 v;
+  v.x = pack_bf16(acc[0] * inv, acc[1] * inv);
+  v.y = pack_bf16(acc[2] * inv, acc[3] * inv);
+  v.z = pack_bf16(acc[4] * inv, acc[5] * inv);
+  v.w = pack_bf16(acc[6] * inv, acc[7] * inv);
+  *reinterpret_cast<uint4*>(a.out + row * DV + d0) = v;
+  if (a.lse && blockIdx.y == 0) a.lse[row] = wsum == 0.f ? -INFINITY : base + logf(wsum);
+}
+
+// How the row tiles are cut into shares.  Times in microseconds, measured on
+// B200: a 64-key tile, a share's start and end (launch, Q, filling the
+// pipeline, writing a partial), the merge kernel.
+constexpr double kTileUs = 0.65, kShareUs = 4., kMergeUs = 4.;
+constexpr int kMinShareTiles = 4;
+
+struct FullPlan {
+  Plan plan;
+  MergePlan merge;
+};
+
+void make_plan(const PrefixMLAArgs& a, FullPlan& f) {
+  Plan& p = f.plan;
+  MergePlan& m = f.merge;
+  m = MergePlan{};
+  const int64_t G = int64_t(a.B) * a.T, rows = G * a.H;
+  if (rows > (int64_t(1) << 31) - 2 * BM || a.P > INT32_MAX - 2 * BN || a.S > (1 << 30))
+    throw std::invalid_argument("shared_prefix_mla: more rows than 32-bit tile indices hold");
+  const int pairs = std::max(1, sm_count() / 2);
+  const int rt = int((rows + BM - 1) / BM);
+  const int prefix_tiles = (a.P + BN - 1) / BN;
+  p.apart = a.S > 0 && a.H % BM != 0;
+  p.tiles = prefix_tiles + (p.apart ? 0 : (a.S + BN - 1) / BN);
+  p.tails = p.apart ? int(G * ((a.H + BM - 1) / BM)) : 0;
+  const bool only_tails = p.apart && a.P == 0;
+  int rest = 0, shares = 1;
+  if (!only_tails) {
+    rest = rt % pairs;
+    p.full = rt - rest;
+    // Equal shares of the rest, one per pair (not shorter than kMinShareTiles), when what the
+    // idle pairs would save exceeds the extra units' cost.
+    const int64_t work = int64_t(rest) * p.tiles;
+    shares = int(std::min<int64_t>(pairs, work / kMinShareTiles));
+    if (shares <= rest || p.tiles * (1. - double(rest) / shares) * kTileUs < (p.apart ? 0. : kShareUs + kMergeUs)) {
+      p.full = rt;
+      rest = 0;
+    }
+  }
+  p.slots = p.apart && !only_tails ? p.full : 0;
+  m.apart = p.apart;
+  m.single = p.slots;
+  m.tile0 = p.apart ? 0 : p.full;
+  m.tiles = only_tails ? 0 : m.single + rest;
+  if (rest) {
+    const int64_t work = int64_t(rest) * p.tiles;
+    // Share i covers flattened tiles [i * work / shares, (i + 1) * work / shares), cut at row tile ends.
+    int64_t pos = 0;
+    int i = 1;
+    for (int t = 0; t < rest; ++t) {
+      m.begin[t] = p.slots;
+      const int64_t end = int64_t(t + 1) * p.tiles;
+      while (pos < end) {
+        while (i * work / shares <= pos) ++i;
+        const int64_t next = std::min(end, i * work / shares);
+        const bool whole = next - pos == p.tiles;
+        Share& s = p.share[p.cut++];
+        s.tile = p.full + t;
+        s.t0 = int(pos - int64_t(t) * p.tiles);
+        s.t1 = int(next - int64_t(t) * p.tiles);
+        s.slot = whole && !p.apart ? -1 : p.slots++;
+        pos = next;
+      }
+    }
+    m.begin[rest] = p.slots;
+    std::sort(p.share, p.share + p.cut, [](const Share& x, const Share& y) { return x.t1 - x.t0 > y.t1 - y.t0; });
+  }
+  if (p.apart && !only_tails) {
+    m.tail_slot0 = p.slots;
+    p.slots += p.tails;
+  }
 }
 
 }  // namespace
 
-void launch_shared_prefix_mla(const PrefixMLAArgs& a, cudaStream_t stream) {
+size_t shared_prefix_mla_scratch_floats(const PrefixMLAArgs& a) {
+  if (int64_t(a.B) * a.T * a.H == 0) return 0;
+  FullPlan f;
+  make_plan(a, f);
+  return size_t(f.plan.slots) * BM * (DV + 1);
+}
+
+void launch_shared_prefix_mla(const PrefixMLAArgs& a, float* scratch, cudaStream_t stream) {
   const int64_t rows = int64_t(a.B) * a.T * a.H;
   if (rows == 0) return;
-  prefix_mla_kernel<<<dim3(unsigned((rows + kWarps - 1) / kWarps)), kWarps * 32, 0, stream>>>(a);
-  cuda_check(cudaGetLastError(), "shared_prefix_mla launch");
+  FullPlan f;
+  make_plan(a, f);
+  const Plan& p = f.plan;
+  static_assert(sizeof(Share) * kMaxShares + 512 < 32764, "kernel parameters");
+  cuda_check(cudaFuncSetAttribute(prefix_mla_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes)),
+             "shared_prefix_mla smem attribute");
+  // Rows past the last one read zeros.  Without a prefix the map covers the queries (never loaded from).
+  const CUtensorMap tq = make_tma_2d(a.q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, uint64_t(rows), D, uint64_t(D) * 2, 64, MC);
+  const CUtensorMap tkv =
+      a.P > 0 ? make_tma_2d(a.prefix, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, uint64_t(a.P), D, uint64_t(a.ld_prefix) * 2, 64, BNC)
+              : make_tma_2d(a.q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, uint64_t(rows), D, uint64_t(D) * 2, 64, BNC);
+  float* part_lse = scratch ? scratch + size_t(p.slots) * BM * DV : nullptr;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * unsigned(p.full + p.cut + p.tails), 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = kSmemBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // the kernel starts with pdl_wait()
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_flag() ? 2 : 1;
+  cuda_check(cudaLaunchKernelEx(&cfg, prefix_mla_kernel, a, p, tq, tkv, a.scale * 1.4426950408889634f, scratch, part_lse),
+             "shared_prefix_mla launch");
+  if (p.slots > 0)
+    launch_pdl(prefix_mla_merge_kernel, dim3(unsigned(f.merge.tiles), DV / 8), dim3(BM), 0, stream,
+               "shared_prefix_mla merge", a, f.merge, static_cast<const float*>(scratch),
+               static_cast<const float*>(part_lse));
 }
 
 }  // namespace b200
