@@ -462,6 +462,7 @@ void sample_tokens(const Tensor& logits, const Tensor& u, const c10::optional<Te
               "sample_tokens: logits FP32 or BF16");
   TORCH_CHECK(logits.dim() == 2 && logits.size(1) >= 1 && (logits.size(1) == 1 || logits.stride(1) == 1) &&
                   logits.stride(0) >= 0, "sample_tokens: logits [R,V], contiguous in the vocabulary");
+  TORCH_CHECK(logits.size(1) <= b200::sample_max_vocabulary(), "sample_tokens: vocabulary too large");
   const int64_t R = logits.size(0);
   auto per_row = [&](const Tensor& t, const char* what) {
     TORCH_CHECK(t.dim() == 1 && t.size(0) == R && t.is_contiguous() && t.device() == logits.device(),
@@ -981,6 +982,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("sparse_mla", &sparse_mla);
   m.def("shared_prefix_mla", &shared_prefix_mla);
   m.def("sample_tokens", &sample_tokens);
+  m.def("sample_max_vocabulary", &b200::sample_max_vocabulary);
   m.def("sparse_mla_scratch_bytes", &sparse_mla_scratch_bytes);
   m.def("sparse_mla_trace", &sparse_mla_trace);
   m.def("topk_trace", &topk_trace);

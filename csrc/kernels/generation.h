@@ -42,6 +42,7 @@ struct SampleArgs {
   int64_t* tokens;  // [R]
   float* logprobs;  // [R]
 };
+int sample_max_vocabulary();
 void launch_sample_tokens(const SampleArgs& a, cudaStream_t stream);
 
 }  // namespace b200

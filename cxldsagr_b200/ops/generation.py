@@ -132,6 +132,8 @@ def sample_tokens(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     if not logits.is_cuda:
         return reference.sample_tokens(logits, u, t_0 if t_t is None else t_t, k_0 if k_t is None else k_t,
                                        p_0 if p_t is None else p_t, m_0 if m_t is None else m_t)
+    if logits.shape[1] > lib().sample_max_vocabulary():
+        raise ValueError(f"the sampling kernel takes vocabularies of up to {lib().sample_max_vocabulary()}")
     if logits.stride(1) != 1 and logits.shape[1] > 1:
         logits = logits.contiguous()
     tokens = torch.empty(R, dtype=torch.int64, device=dev)
