@@ -9,17 +9,19 @@
 // The masses are whole numbers, so sums do not depend on their order: a draw
 // is the same whatever the batch, the split over threads or the kernel.
 //
-// One cluster of 1 to 16 CTAs per row: a row of 129,280 FP32 logits (517 KB)
-// is read from HBM once, in slices that stay in the CTAs' shared memory for all
-// later passes.  The order is never sorted: a histogram of d (2,048 bins over
-// the range where W > 0, counts and masses) finds the bin in which a filter
-// cuts, and the few entries of that bin are ranked against each other.  A bin
-// with more entries than fit the list (equal logits) is split again by the bits
-// of the logits until it fits or holds one value, which is cut by index.
+// The order is never sorted: a histogram of d (1,024 bins, counts and masses)
+// finds the bins in which the filters cut, and the few entries of those bins
+// are ranked against each other.  When they do not fit the list (equal or
+// clustered logits), the bin is split again by the bits of the logits until it
+// fits or holds one value, which is cut by index.
 //
-// Sums over the cluster go through distributed shared memory; every CTA merges
-// and scans 1 / C of the histogram's bins.  Nothing spins: the CTAs meet at
-// hardware cluster barriers only.
+// A row belongs to a cluster of 1 to 16 CTAs: it is read from HBM once and
+// stays in their shared memory for all later passes (first as logits, then as
+// d).  The CTAs exchange values through distributed shared memory.  Nothing
+// spins: they meet at hardware barriers only (six per row with one filter, two without).
+#include <algorithm>
+#include <cmath>
+
 #include "../common/host.h"
 #include "../common/ptx.cuh"
 #include "generation.h"
@@ -30,33 +32,51 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 16;
-// A warp's share of a slice is at most 32 blocks of 32 entries; a bin's 18-bit halves of up to
-// 16,383 masses fit 32 bits.
-constexpr int kMaxSlice = 16352;
-constexpr int kBins = 2048;
+constexpr int kStep = 128;               // positions per warp step (4 per lane)
+constexpr int kSubs = 4;                 // parts of a warp's positions whose kept masses are summed apart
+constexpr int kSlice = 16384;            // positions of a CTA, at most (16 of them padding at least)
+constexpr int kBins = 1024;
 constexpr int kList = 512;
 constexpr float kFixed = 68719476736.f;  // 2^36
-constexpr float kHalf = 262144.f;        // 2^18
 constexpr float kSpan = 25.f;            // exp(-25) * 2^36 < 1: entries further down have no mass
+constexpr float kTiny = 0x1p-60f;        // distances below it are told apart by their logits
 constexpr uint64_t kNothing = ~0ull;     // composite above every entry
+constexpr uint64_t kInK = 1ull << 63, kInP = 1ull << 62;  // list entry belongs to the bin(s) of the top-k / top-p cut
+constexpr uint64_t kMassBits = kInP - 1;
+static_assert(kBins == 2 * kThreads, "two bins per thread");
 
 struct alignas(16) Shared {
-  uint64_t xch[2][4][kMaxCluster];  // exchanged values (double buffered)
-  uint64_t red[kWarps];
-  uint64_t wsum[kWarps];
-  uint64_t decision[2][4];          // written by the CTA that owns the cut (double buffered)
-  uint64_t list[kList];             // CTA 0: entries of the cut bin
-  uint64_t list_mass[kList];
-  uint32_t list_count;
-  uint32_t cnt[kBins], lo[kBins], hi[kBins];
+  uint64_t xch[2][2][kMaxCluster];  // exchanged values (double buffered)
+  uint64_t decision[2];             // written by the CTA that owns an equal-value cut (double buffered)
+  uint64_t red[2][kWarps];
+  uint32_t red32[2][kWarps];
+  uint64_t sub[kWarps * kSubs];     // kept masses
+  uint64_t found[4];                // bin of a cut and what lies before it
+  uint32_t list_count[4];           // CTA 0: entries listed by each gather
+  uint32_t own_count, own_base;
+  uint32_t own[kList];              // this CTA's part of the list: positions
+  uint64_t own_mass[kList];         // ... and for top-p, the mass before each
+  union {
+    ulonglong2 list[kList];         // the row's entries in the cut bins: composite, mass with its group bits
+    struct {
+      uint64_t mass[kThreads];
+      uint32_t cnt[kThreads];
+    } part;                         // merge: partial sums
+  };
+  uint32_t cnt[kBins], lo[kBins], hi[kBins];  // this CTA's histogram (masses in halves)
+  uint32_t all_cnt[kBins];          // the row's
+  uint64_t all_mass[kBins];
 };
 
-__device__ __forceinline__ void cluster_sync_all() {
-  __syncwarp();
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 __device__ __forceinline__ void remote_st64(const void* local, uint32_t rank, uint64_t v) {
   asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(mapa_shared(smem_u32(local), rank)), "l"(v) : "memory");
+}
+__device__ __forceinline__ void remote_st32(const void* local, uint32_t rank, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapa_shared(smem_u32(local), rank)), "r"(v) : "memory");
+}
+__device__ __forceinline__ void remote_st128(const void* local, uint32_t rank, uint64_t a, uint64_t b) {
+  asm volatile("st.shared::cluster.v2.u64 [%0], {%1, %2};" ::"r"(mapa_shared(smem_u32(local), rank)), "l"(a), "l"(b)
+               : "memory");
 }
 __device__ __forceinline__ uint32_t remote_ld32(const void* local, uint32_t rank) {
   uint32_t v;
@@ -83,20 +103,10 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 __device__ __forceinline__ uint64_t composite(float x, int index) {
   return (uint64_t(order_key(x)) << 32) | uint32_t(~index);
 }
+__device__ __forceinline__ float clean(float x) { return x == x ? x + 0.f : -INFINITY; }  // NaN: masked; -0: +0
 
-// floor(2^36 w), w in [0, 1], as 2^18 hi + lo: the truncations are additions of 2^23 rounded to zero.
-__device__ __forceinline__ void mass_halves(float w, uint32_t& hi, uint32_t& lo) {
-  const float s = w * kHalf;
-  const float t = __fadd_rz(s, 8388608.f);
-  hi = __float_as_uint(t) & 0x7fffffu;
-  const float rest = s - (t - 8388608.f);  // exact, in [0, 1)
-  lo = __float_as_uint(__fadd_rz(rest * kHalf, 8388608.f)) & 0x7fffffu;
-}
-__device__ __forceinline__ uint64_t mass_of(float w) {
-  uint32_t hi, lo;
-  mass_halves(w, hi, lo);
-  return (uint64_t(hi) << 18) + lo;
-}
+// floor(2^36 w); 0 for NaN and for weights below 2^-36.
+__device__ __forceinline__ uint64_t mass_of(float w) { return uint64_t(fmaxf(w, 0.f) * kFixed); }
 
 __device__ __forceinline__ uint64_t warp_sum64(uint64_t v) {
 #pragma unroll
@@ -113,52 +123,94 @@ __device__ __forceinline__ uint64_t warp_inclusive64(uint64_t v) {
   return v;
 }
 
+// A row as one CTA of its cluster sees it.  Positions [0, chunk * kWarps) cover
+// the CTA's slice of the row (index = begin + position) with some padding;
+// warp w owns [w * chunk, + chunk).  NaN logits and padding turn into a d that
+// no comparison accepts.
 template <bool BF16>
 struct Row {
   Shared& s;
-  float* v;  // the slice: logits, then d, then the kept weights
+  float* v;                // logits, then d
   const void* src;
-  int V, C, rank, begin, n;
-  int chunk, w0, w1;  // this warp's entries of the slice
-  float mx, T;
-  int first;          // index of the best token
-  int phase = 0, event = 0;  // exchange and decision buffers
+  int C, rank;
+  int begin, start, stop;  // index of position 0; the slice's entries are [start, stop)
+  int w0, w1, sub;         // this warp's positions, in parts of `sub`
+  float mx, T, inv, scale; // scale: a power of two applied to logit differences and T, 1 for usual rows
+  int phase = 0, turn = 0, event = 0, gathers = 0;  // buffers in use
 
   __device__ Row(Shared& s_) : s(s_) {}
 
   __device__ float logit(int i) const {
-    float x;
-    if constexpr (BF16) x = __bfloat162float(static_cast<const __nv_bfloat16*>(src)[i]);
-    else x = static_cast<const float*>(src)[i];
-    return x == x ? x + 0.f : -INFINITY;  // NaN counts as masked; -0 as +0
+    if constexpr (BF16) return clean(__bfloat162float(static_cast<const __nv_bfloat16*>(src)[i]));
+    else return clean(static_cast<const float*>(src)[i]);
   }
-  // d of a logit; -inf stays -inf whatever T is.
-  __device__ float dist(float x) const { return x == mx ? 0.f : x == -INFINITY ? -INFINITY : (x - mx) / T; }
+  __device__ float at(int j) const {  // the logit at a position, from memory
+    const int i = begin + j;
+    return i >= start && i < stop ? logit(i) : -INFINITY;
+  }
+  __device__ float4& quad(int j) const { return *reinterpret_cast<float4*>(&v[j]); }
+  // a / T.  Markstein's quotient: a * inv with inv the rounded reciprocal is within 2 units in the last
+  // place, and one correction by its exact remainder leaves an error of 2^-47 of the quotient before the
+  // final rounding.  It needs normal numbers: T lies within 2^+-40 (the row is scaled otherwise), and
+  // quotients below kTiny are not trusted with an order.
+  __device__ float quotient(float a) const {
+    const float q = a * inv;
+    return fmaf(fmaf(-q, T, a), inv, q);
+  }
+  __device__ float dist(float x) const { return quotient(x == mx ? 0.f : (x - mx) * scale); }
   __device__ static float weight(float d) { return expf(d); }
-  __device__ static int bin(float d) { return min(kBins - 1, int(-d * (kBins / kSpan))); }
 
-  // Sum over the CTA (every thread gets it).
-  __device__ uint64_t block_sum(uint64_t x) {
-    x = warp_sum64(x);
-    __syncthreads();
-    if (threadIdx.x % 32 == 0) s.red[threadIdx.x / 32] = x;
-    __syncthreads();
-    uint64_t t = 0;
-#pragma unroll
-    for (int i = 0; i < kWarps; ++i) t += s.red[i];
-    return t;
+  // f(j, d) for four positions per lane and step.
+  template <typename F>
+  __device__ void sweep(int j0, int j1, F&& f) const {
+    for (int j = j0 + 4 * int(threadIdx.x % 32); j < j1; j += kStep) {
+      const float4 q = quad(j);
+      const float d[4] = {q.x, q.y, q.z, q.w};
+      f(j, d);
+    }
   }
+  // The same while the logits are replaced by their distances (base: the best logit, 0 in a scaled row).
+  template <typename F>
+  __device__ void first_sweep(int j0, int j1, float base, F&& f) {
+    for (int j = j0 + 4 * int(threadIdx.x % 32); j < j1; j += kStep) {
+      const float4 q = quad(j);
+      const float d[4] = {quotient(q.x - base), quotient(q.y - base), quotient(q.z - base), quotient(q.w - base)};
+      quad(j) = make_float4(d[0], d[1], d[2], d[3]);
+      f(j, d);
+    }
+  }
+
+  // ------------------------------------------------ the CTA and the cluster
+  __device__ void cluster_sync() const {
+    if (C == 1) {
+      __syncthreads();
+    } else {
+      __syncwarp();
+      asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+  }
+  // Reductions over the CTA; every thread gets the result.
   template <typename Op>
   __device__ uint64_t block_pick(uint64_t x, Op op) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) x = op(x, __shfl_xor_sync(0xffffffffu, x, o));
+    uint64_t* red = s.red[turn];
+    turn ^= 1;
+    if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = x;
     __syncthreads();
-    if (threadIdx.x % 32 == 0) s.red[threadIdx.x / 32] = x;
-    __syncthreads();
-    uint64_t t = s.red[0];
+    x = red[threadIdx.x % kWarps];
 #pragma unroll
-    for (int i = 1; i < kWarps; ++i) t = op(t, s.red[i]);
-    return t;
+    for (int o = kWarps / 2; o; o >>= 1) x = op(x, __shfl_xor_sync(0xffffffffu, x, o));
+    return x;
+  }
+  __device__ uint64_t block_max(uint64_t x) {
+    return block_pick(x, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
+  }
+  __device__ uint64_t block_min(uint64_t x) {
+    return block_pick(x, [](uint64_t a, uint64_t b) { return a < b ? a : b; });
+  }
+  __device__ uint64_t block_sum(uint64_t x) {
+    return block_pick(x, [](uint64_t a, uint64_t b) { return a + b; });
   }
   // Hand `a` (and `b`) of every CTA to every CTA; the values are uniform in the CTA.
   __device__ const uint64_t (*exchange(uint64_t a, uint64_t b = 0))[kMaxCluster] {
@@ -168,103 +220,110 @@ struct Row {
       remote_st64(&x[0][rank], threadIdx.x, a);
       remote_st64(&x[1][rank], threadIdx.x, b);
     }
-    cluster_sync_all();
+    cluster_sync();
     return x;
-  }
-  // One thread of the cluster tells every CTA; all read after `decided()`.
-  __device__ void decide(uint64_t a, uint64_t b = 0, uint64_t c = 0, uint64_t d = 0) {
-    for (int q = 0; q < C; ++q) {
-      remote_st64(&s.decision[event][0], q, a);
-      remote_st64(&s.decision[event][1], q, b);
-      remote_st64(&s.decision[event][2], q, c);
-      remote_st64(&s.decision[event][3], q, d);
-    }
-  }
-  __device__ const uint64_t* decided() {
-    cluster_sync_all();
-    const uint64_t* d = s.decision[event];
-    event ^= 1;
-    return d;
-  }
-
-  // First local index whose cumulative weight in index order exceeds r, in the
-  // warp that holds it (the weights before the warp's chunk sum to warp_before).
-  template <typename W>
-  __device__ int select_in_warp(W&& weight_at, uint64_t r, uint64_t warp_before) {
-    const int lane = threadIdx.x % 32;
-    uint64_t mine = 0;
-    for (int t = 0; t < 32; ++t) {
-      const int j = w0 + lane * 32 + ((lane + t) & 31);
-      if (j < w1) mine += weight_at(j);
-    }
-    const uint64_t inc = warp_inclusive64(mine);
-    const uint32_t over = __ballot_sync(0xffffffffu, warp_before + inc > r);
-    const int block = __ffs(over) - 1;
-    const uint64_t before = warp_before + __shfl_sync(0xffffffffu, inc - mine, block);
-    const int j = w0 + block * 32 + lane;
-    const uint64_t e = warp_inclusive64(j < w1 ? weight_at(j) : 0);
-    const uint32_t hit = __ballot_sync(0xffffffffu, before + e > r);
-    return w0 + block * 32 + __ffs(hit) - 1;
   }
 
   // ---------------------------------------------------------------- cuts
-  // Histogram over the entries whose (bin, mass) `entry(j, b, w)` gives; merged over the cluster, CTA c
-  // ends up with the bins [c, c + 1) * kBins / C (masses as 64 bits in hi:lo).
-  template <typename F>
-  __device__ void histogram(F&& entry, bool masses) {
+  __device__ void clear_histogram() {
     for (int b = threadIdx.x; b < kBins; b += kThreads) s.cnt[b] = s.lo[b] = s.hi[b] = 0;
     __syncthreads();
-    const int lane = threadIdx.x % 32;
-    for (int j = w0 + lane; j < w1; j += 32) {
+  }
+  // In halves of 18 bits: sums of 16,384 of them fit a word, and no addition waits for a carry.
+  __device__ void add_mass(int b, uint64_t m) {
+    atomicAdd(&s.hi[b], uint32_t(m >> 18));
+    atomicAdd(&s.lo[b], uint32_t(m) & 0x3ffffu);
+  }
+  // CTA c sums the bins [c, c + 1) * kBins / C of all CTAs and hands them to all; every thread then holds
+  // what lies before its two bins.
+  __device__ void merge() {
+    cluster_sync();
+    if (C == 1) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int b = 2 * threadIdx.x + i;
+        s.all_cnt[b] = s.cnt[b];
+        s.all_mass[b] = (uint64_t(s.hi[b]) << 18) + s.lo[b];
+      }
+    } else {
+      // `per` neighbouring threads take neighbouring bins; groups of threads share the sources.
+      const int per = kBins / C, groups = kThreads / per, g = threadIdx.x / per;
+      const int b = rank * per + threadIdx.x % per;
+      uint32_t c = 0;
+      uint64_t m = 0;
+#pragma unroll 2
+      for (int q = g; q < C; q += groups) {
+        c += remote_ld32(&s.cnt[b], q);
+        m += (uint64_t(remote_ld32(&s.hi[b], q)) << 18) + remote_ld32(&s.lo[b], q);
+      }
+      s.part.mass[threadIdx.x] = m;
+      s.part.cnt[threadIdx.x] = c;
+      __syncthreads();
+      c = 0;
+      m = 0;
+      for (int i = 0; i < groups; ++i) {
+        m += s.part.mass[i * per + threadIdx.x % per];
+        c += s.part.cnt[i * per + threadIdx.x % per];
+      }
+#pragma unroll 2
+      for (int q = g; q < C; q += groups) {
+        remote_st32(&s.all_cnt[b], q, c);
+        remote_st64(&s.all_mass[b], q, m);
+      }
+      cluster_sync();
+    }
+    scan();
+  }
+  uint32_t before_cnt;              // in the bins before the thread's two
+  uint64_t before_mass;
+  uint64_t total_count, total_mass;
+  __device__ void scan() {  // (the thread's own bins were written by itself when C == 1)
+    const int b = 2 * threadIdx.x, warp = threadIdx.x / 32;
+    const uint32_t c = s.all_cnt[b] + s.all_cnt[b + 1];
+    const uint64_t m = s.all_mass[b] + s.all_mass[b + 1];
+    const uint64_t mi = warp_inclusive64(m);
+    uint32_t ci = c;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const uint32_t n = __shfl_up_sync(0xffffffffu, ci, o);
+      if (int(threadIdx.x % 32) >= o) ci += n;
+    }
+    uint64_t* red = s.red[turn];
+    uint32_t* red32 = s.red32[turn];
+    turn ^= 1;
+    if (threadIdx.x % 32 == 31) {
+      red[warp] = mi;
+      red32[warp] = ci;
+    }
+    __syncthreads();
+    before_cnt = ci - c;
+    before_mass = mi - m;
+    total_count = total_mass = 0;
+#pragma unroll 4
+    for (int i = 0; i < kWarps; ++i) {
+      if (i == warp) {
+        before_cnt += uint32_t(total_count);
+        before_mass += total_mass;
+      }
+      total_count += red32[i];
+      total_mass += red[i];
+    }
+  }
+  template <typename F>
+  __device__ void histogram(F&& entry) {
+    clear_histogram();
+    for (int j = w0 + int(threadIdx.x % 32); j < w1; j += 32) {
       int b;
       float w;
       if (entry(j, b, w)) {
         atomicAdd(&s.cnt[b], 1u);
-        if (masses) {
-          uint32_t h, l;
-          mass_halves(w, h, l);
-          atomicAdd(&s.hi[b], h);
-          atomicAdd(&s.lo[b], l);
-        }
+        add_mass(b, mass_of(w));
       }
     }
-    cluster_sync_all();
-    const int per = kBins / C;
-    for (int b = rank * per + threadIdx.x; b < (rank + 1) * per; b += kThreads) {
-      uint32_t c = 0;
-      uint64_t m = 0;
-      for (int q = 0; q < C; ++q) {
-        c += remote_ld32(&s.cnt[b], q);
-        if (masses) m += (uint64_t(remote_ld32(&s.hi[b], q)) << 18) + remote_ld32(&s.lo[b], q);
-      }
-      s.cnt[b] = c;
-      s.lo[b] = uint32_t(m);
-      s.hi[b] = uint32_t(m >> 32);
-    }
-    // The segment is only read by this CTA from here on.
-    __syncthreads();
-    uint64_t c = 0, m = 0;
-    for (int b = rank * per + threadIdx.x; b < (rank + 1) * per; b += kThreads) {
-      c += s.cnt[b];
-      m += (uint64_t(s.hi[b]) << 32) | s.lo[b];
-    }
-    seg_count = block_sum(c);
-    seg_mass = block_sum(m);
-    const uint64_t(*x)[kMaxCluster] = exchange(seg_count, seg_mass);
-    count_before = mass_before = total_count = total_mass = 0;
-    for (int q = 0; q < C; ++q) {
-      if (q < rank) {
-        count_before += x[0][q];
-        mass_before += x[1][q];
-      }
-      total_count += x[0][q];
-      total_mass += x[1][q];
-    }
+    merge();
   }
-  uint64_t seg_count, seg_mass, count_before, mass_before, total_count, total_mass;
 
-  // What a cut looks for: the first bin where the count (top-k) or the mass
-  // (top-p), added to what lies before the histogram, reaches its goal.
+  // What a cut looks for: the first bin (entry) at which the count (top-k) or the mass (top-p) reaches its goal.
   struct Goal {
     bool by_mass;
     uint64_t k;
@@ -275,136 +334,172 @@ struct Row {
   };
   struct Cut {
     int bin;
-    uint64_t count, mass, entries;  // before the bin; entries in it
+    uint64_t count, mass;          // before the bin
+    uint64_t entries, bin_mass;    // in it
   };
-  // The goal is reached within this histogram (count0 / mass0 lie before it).
-  __device__ Cut find_bin(const Goal& g, uint64_t count0, uint64_t mass0) {
-    const uint64_t cb = count0 + count_before, mb = mass0 + mass_before;
-    if (!g.reached(cb, mb) && g.reached(cb + seg_count, mb + seg_mass)) {  // in this CTA's segment
-      const int per = kBins / C, q = (per + kThreads - 1) / kThreads;
-      const int b0 = rank * per + threadIdx.x * q, b1 = min(b0 + q, (rank + 1) * per);
-      uint64_t c = 0, m = 0;
-      for (int b = b0; b < b1; ++b) {
-        c += s.cnt[b];
-        m += (uint64_t(s.hi[b]) << 32) | s.lo[b];
+  // The bin of the row's histogram in which the goal is reached (-1: in none); count0 / mass0 lie before it.
+  __device__ Cut find_bin(const Goal& g, uint64_t count0 = 0, uint64_t mass0 = 0) {
+    __syncthreads();  // `found` of the call before has been read
+    if (threadIdx.x == 0) s.found[0] = kNothing;
+    __syncthreads();
+    uint64_t c = count0 + before_cnt, m = mass0 + before_mass;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int b = 2 * threadIdx.x + i;
+      const uint64_t ce = c + s.all_cnt[b], me = m + s.all_mass[b];
+      if (!g.reached(c, m) && g.reached(ce, me)) {
+        s.found[0] = b;
+        s.found[1] = c;
+        s.found[2] = m;
       }
-      const uint64_t ci = warp_inclusive64(c), mi = warp_inclusive64(m);
-      __syncthreads();
-      if (threadIdx.x % 32 == 31) {
-        s.red[threadIdx.x / 32] = ci;
-        s.wsum[threadIdx.x / 32] = mi;
-      }
-      __syncthreads();
-      uint64_t cs = cb + ci - c, ms = mb + mi - m;
-      for (int i = 0; i < int(threadIdx.x / 32); ++i) {
-        cs += s.red[i];
-        ms += s.wsum[i];
-      }
-      for (int b = b0; b < b1; ++b) {
-        const uint64_t ce = cs + s.cnt[b], me = ms + ((uint64_t(s.hi[b]) << 32) | s.lo[b]);
-        if (!g.reached(cs, ms) && g.reached(ce, me)) decide(uint64_t(b), cs, ms, s.cnt[b]);
-        cs = ce;
-        ms = me;
-      }
+      c = ce;
+      m = me;
     }
-    const uint64_t* d = decided();
-    return Cut{int(d[0]), d[1], d[2], d[3]};
+    __syncthreads();
+    Cut r;
+    r.bin = int(int64_t(s.found[0]));
+    r.count = s.found[1];
+    r.mass = s.found[2];
+    r.entries = r.bin >= 0 ? s.all_cnt[r.bin] : 0;
+    r.bin_mass = r.bin >= 0 ? s.all_mass[r.bin] : 0;
+    return r;
   }
 
-  // Gather the entries that pass `in(j)` (at most kList) into CTA 0's list, rank them and return the
-  // composite of the last kept one (kNothing: none) and the mass through it.
-  template <typename F>
-  __device__ uint64_t rank_list(F&& in, const Goal& g, const Cut& c, uint64_t floor_, uint64_t& mass_through) {
-    if (threadIdx.x == 0) s.list_count = 0;
-    cluster_sync_all();
+  // A pass that lists entries: each(d) returns the mass of a surely kept position (0: none) and
+  // sets `want` to list it.  The sums of masses go to s.sub.  Afterwards every CTA holds the row's list, up to
+  // kList entries (group(x) gives an entry's group bits); returns their number in the row.
+  template <typename F, typename G>
+  __device__ int gather(F&& each, G&& group) {
+    if (threadIdx.x == 0) s.own_count = 0;
+    __syncthreads();
     const int lane = threadIdx.x % 32;
-    for (int jb = w0; jb < w1; jb += 32) {
-      const int j = jb + lane;
-      const bool take = j < w1 && in(j);
-      const uint32_t m = __ballot_sync(0xffffffffu, take);
-      if (!m) continue;
-      uint32_t at = 0;
-      if (lane == 0) at = remote_add32(&s.list_count, 0, __popc(m));
-      at = __shfl_sync(0xffffffffu, at, 0) + __popc(m & ((1u << lane) - 1));
-      if (take && at < kList) {
-        const float x = logit(begin + j);
-        remote_st64(&s.list[at], 0, composite(x, begin + j));
-        remote_st64(&s.list_mass[at], 0, mass_of(weight(dist(x))));
-      }
-    }
-    cluster_sync_all();
-    if (rank == 0) {
-      // Warp w ranks entries w, w + 16, ...: what lies before each in the order.
-      const int m = min(int(s.list_count), kList);
-      uint64_t last = kNothing, through = c.mass;
-      for (int e = threadIdx.x / 32; e < m; e += kWarps) {
-        const uint64_t mine = s.list[e];
-        uint64_t cnt = 0, mass = 0;
-        for (int f = lane; f < m; f += 32)
-          if (s.list[f] > mine) {
-            ++cnt;
-            mass += s.list_mass[f];
+    for (int i = 0; i < kSubs; ++i) {
+      uint64_t m = 0;
+      sweep(w0 + i * sub, min(w1, w0 + (i + 1) * sub), [&](int j, const float (&d)[4]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          bool want = false;
+          m += each(d[e], want);
+          if (want) {
+            const uint32_t slot = atomicAdd(&s.own_count, 1u);
+            if (slot < kList) s.own[slot] = j + e;
           }
-        cnt = c.count + warp_sum64(cnt);
-        mass = c.mass + warp_sum64(mass);
-        if (!g.reached(cnt, mass) && mine >= floor_) {
-          last = min(last, mine);
-          through = max(through, mass + s.list_mass[e]);
+        }
+      });
+      m = warp_sum64(m);
+      if (lane == 0) s.sub[threadIdx.x / 32 * kSubs + i] = m;
+    }
+    __syncthreads();
+    const int n = s.own_count;
+    const uint32_t* counter = &s.list_count[gathers++];
+    if (threadIdx.x == 0 && n) s.own_base = remote_add32(counter, 0, n);
+    __syncthreads();
+    // (entry, destination) pairs over the threads.
+    for (int e = threadIdx.x; e < min(n, kList) * C; e += kThreads) {
+      const int j = s.own[e / C];
+      const float x = at(j);
+      const uint32_t slot = s.own_base + e / C;
+      if (slot < kList) remote_st128(&s.list[slot], e % C, composite(x, begin + j), mass_of(weight(dist(x))) | group(x));
+    }
+    cluster_sync();
+    return int(remote_ld32(counter, 0));
+  }
+  // The cut among the n <= kList listed entries: warp w ranks this CTA's entries w, w + 16, ... against the
+  // row's, the results meet in an exchange (two when a top-p goal waits for the mass that top-k leaves).
+  // Returns the composite of the last kept entry; `through`: the mass through the top-k cut, in and out.
+  __device__ uint64_t rank_list(int n, bool by_k, const Goal& gk, const Cut& ck, bool by_p, float p, const Cut& cp,
+                                uint64_t& through) {
+    const int lane = threadIdx.x % 32, own = s.own_count;
+    const uint32_t base = s.own_base;
+    uint64_t last = kNothing, mass_k = 0;
+    for (int e = threadIdx.x / 32; e < own; e += kWarps) {
+      const ulonglong2 mine = s.list[base + e];
+      uint32_t cnt = 0;
+      uint64_t mk = 0, mp = 0;
+      for (int f = lane; f < n; f += 32) {
+        const ulonglong2 o = s.list[f];
+        if (o.x > mine.x) {
+          const uint64_t m = o.y & kMassBits;
+          if (o.y & kInK) {
+            ++cnt;
+            mk += m;
+          }
+          if (o.y & kInP) mp += m;
         }
       }
-      last = block_pick(last, [](uint64_t a, uint64_t b) { return a < b ? a : b; });
-      through = block_pick(through, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
-      if (threadIdx.x == 0) decide(last, through);
+      if (by_k) {
+        cnt = __reduce_add_sync(0xffffffffu, cnt);
+        mk = ck.mass + warp_sum64(mk);
+        if ((mine.y & kInK) && !gk.reached(ck.count + cnt, mk)) {
+          last = min(last, uint64_t(mine.x));
+          mass_k = max(mass_k, mk + uint64_t(mine.y & kMassBits));
+        }
+      }
+      if (by_p) {
+        mp = warp_sum64(mp);
+        if (lane == 0) s.own_mass[e] = (mine.y & kInP) ? cp.mass + mp : kNothing;
+      }
     }
-    const uint64_t* d = decided();
-    mass_through = d[1];
-    return d[0];
+    uint64_t cut = 0;
+    if (by_k) {
+      const uint64_t(*x)[kMaxCluster] = exchange(block_min(last), block_max(mass_k));
+      cut = kNothing;
+      through = 0;
+      for (int q = 0; q < C; ++q) {
+        cut = min(cut, x[0][q]);
+        through = max(through, x[1][q]);
+      }
+    }
+    if (by_p) {
+      const double want = double(p) * double(through);
+      __syncthreads();
+      last = kNothing;
+      for (int e = threadIdx.x; e < own; e += kThreads)
+        if (s.own_mass[e] != kNothing && double(s.own_mass[e]) < want) last = min(last, uint64_t(s.list[base + e].x));
+      const uint64_t(*x)[kMaxCluster] = exchange(block_min(last));
+      last = kNothing;
+      for (int q = 0; q < C; ++q) last = min(last, x[0][q]);
+      cut = max(cut, last);
+    }
+    return cut;
   }
 
-  // The last kept entry of a goal (composite; entries of composite >= it are kept) and the mass through
-  // it.  `floor_`: an earlier cut that also holds.  The histogram of d must be built.
-  __device__ uint64_t find_cut(const Goal& g, uint64_t floor_, uint64_t& mass_through, bool& rebuilt) {
-    Cut c = find_bin(g, 0, 0);
-    if (c.entries <= kList)
-      return rank_list([&](int j) { return v[j] > -kSpan && bin(v[j]) == c.bin; }, g, c, floor_, mass_through);
-    // Too many: split by the keys' bits inside the bin.  Any entry between the
-    // bin's lowest and highest key belongs to it (d is monotone in x).
-    rebuilt = true;
+  // The slow way for a bin whose entries do not fit the list: split it by the keys' bits.  `in` tells
+  // whether a logit belongs to the bin; any entry between the bin's lowest and highest key does (d is
+  // monotone in x).
+  template <typename F>
+  __device__ uint64_t find_cut(F&& in, Cut c, const Goal& g, uint64_t& through) {
+    const int lane = threadIdx.x % 32;
     uint64_t top = 0, low = kNothing;
-    for (int j = w0 + int(threadIdx.x % 32); j < w1; j += 32)
-      if (v[j] > -kSpan && bin(v[j]) == c.bin) {
-        const uint64_t k = order_key(logit(begin + j));
+    for (int j = w0 + lane; j < w1; j += 32) {
+      const float x = at(j);
+      if (in(x)) {
+        const uint64_t k = order_key(x);
         top = max(top, k);
         low = min(low, k);
       }
+    }
     while (true) {
-      top = block_pick(top, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
-      low = block_pick(low, [](uint64_t a, uint64_t b) { return a < b ? a : b; });
+      top = block_max(top);
+      low = block_min(low);
       const uint64_t(*x)[kMaxCluster] = exchange(top, low);
       for (int q = 0; q < C; ++q) {
         top = max(top, x[0][q]);
         low = min(low, x[1][q]);
       }
       const uint32_t khi = uint32_t(top), klo = uint32_t(low);
-      auto inside = [&](int j) {
-        const uint32_t k = order_key(logit(begin + j));
-        return k >= klo && k <= khi;
-      };
-      if (c.entries <= kList) return rank_list(inside, g, c, floor_, mass_through);
-      if (khi == klo) return cut_equal(khi, g, c, floor_, mass_through);
+      if (khi == klo) return cut_equal(khi, g, c, through);
       int shift = 0;
       while (((khi - klo) >> shift) >= uint32_t(kBins)) ++shift;
       const uint64_t count0 = c.count, mass0 = c.mass;
-      histogram(
-          [&](int j, int& b, float& w) {
-            const float xv = logit(begin + j);
-            const uint32_t k = order_key(xv);
-            if (k < klo || k > khi) return false;
-            b = int((khi - k) >> shift);
-            w = weight(dist(xv));
-            return true;
-          },
-          true);
+      histogram([&](int j, int& b, float& w) {
+        const float xv = at(j);
+        const uint32_t k = order_key(xv);
+        if (k < klo || k > khi) return false;
+        b = int((khi - k) >> shift);
+        w = weight(dist(xv));
+        return true;
+      });
       c = find_bin(g, count0, mass0);
       // The bin's own lowest and highest keys.
       const uint32_t h = khi - (uint32_t(c.bin) << shift);
@@ -412,8 +507,8 @@ struct Row {
       const uint32_t l = h - klo > span ? h - span : klo;
       top = 0;
       low = kNothing;
-      for (int j = w0 + int(threadIdx.x % 32); j < w1; j += 32) {
-        const uint64_t k = order_key(logit(begin + j));
+      for (int j = w0 + lane; j < w1; j += 32) {
+        const uint64_t k = order_key(at(j));
         if (k >= l && k <= h) {
           top = max(top, k);
           low = min(low, k);
@@ -423,7 +518,8 @@ struct Row {
   }
 
   // Many entries of one value: the goal keeps the first m of them in index order.
-  __device__ uint64_t cut_equal(uint32_t key, const Goal& g, const Cut& c, uint64_t floor_, uint64_t& mass_through) {
+  __device__ uint64_t cut_equal(uint32_t key, const Goal& g, const Cut& c, uint64_t& through) {
+    const int lane = threadIdx.x % 32;
     const uint64_t one = mass_of(weight(dist(key_value(key))));
     uint64_t m;
     if (g.by_mass) {
@@ -433,187 +529,306 @@ struct Row {
     } else {
       m = g.k - c.count;
     }
-    auto equal = [&](int j) { return uint64_t(order_key(logit(begin + j)) == key); };
     uint64_t mine = 0;
-    for (int j = w0 + int(threadIdx.x % 32); j < w1; j += 32) mine += equal(j);
+    for (int j = w0 + lane; j < w1; j += 32) mine += order_key(at(j)) == key;
     mine = warp_sum64(mine);
-    const uint64_t total = block_sum(threadIdx.x % 32 == 0 ? mine : 0);
-    if (threadIdx.x % 32 == 0) s.wsum[threadIdx.x / 32] = mine;
-    const uint64_t(*x)[kMaxCluster] = exchange(total);
+    if (lane == 0) s.sub[threadIdx.x / 32] = mine;
+    const uint64_t(*x)[kMaxCluster] = exchange(block_sum(lane == 0 ? mine : 0));
     uint64_t before = 0;
     for (int q = 0; q < rank; ++q) before += x[0][q];
-    for (int i = 0; i < int(threadIdx.x / 32); ++i) before += s.wsum[i];
+    for (int i = 0; i < int(threadIdx.x / 32); ++i) before += s.sub[i];
     if (m - 1 >= before && m - 1 < before + mine) {  // this warp holds the m-th one
-      const int j = select_in_warp(equal, m - 1, before);
-      if (threadIdx.x % 32 == 0) decide(composite(key_value(key), begin + j));
+      uint32_t left = uint32_t(m - 1 - before);      // equal ones before it here
+      for (int j0 = w0; j0 < w1; j0 += 32) {
+        const uint32_t eq = __ballot_sync(0xffffffffu, order_key(at(j0 + lane)) == key);
+        const uint32_t n = __popc(eq);
+        if (left < n) {
+          if (((eq >> lane) & 1u) && __popc(eq & ((1u << lane) - 1)) == left)
+            for (int q = 0; q < C; ++q) remote_st64(&s.decision[event], q, composite(key_value(key), begin + j0 + lane));
+          break;
+        }
+        left -= n;
+      }
     }
-    mass_through = c.mass + m * one;
-    return max(decided()[0], floor_);
+    cluster_sync();
+    through = c.mass + m * one;
+    const uint64_t cut = s.decision[event];
+    event ^= 1;
+    return cut;
   }
 };
 
 template <bool BF16>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant__ SampleArgs a, int C) {
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_constant__ SampleArgs a, int C, int chunk) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   pdl_trigger();
   pdl_wait();
   Shared& s = *reinterpret_cast<Shared*>(smem_raw);
+  using R = Row<BF16>;
   constexpr int VEC = BF16 ? 8 : 4;
   constexpr int kSize = BF16 ? 2 : 4;
   const int64_t row = blockIdx.x / C;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  Row<BF16> r(s);
+  R r(s);
   r.C = C;
-  r.V = a.V;
-  r.rank = int(cluster_ctarank());
+  r.rank = int(blockIdx.x % C);
   r.src = static_cast<const uint8_t*>(a.logits) + row * a.ld * kSize;
+  r.v = reinterpret_cast<float*>(smem_raw + sizeof(Shared));
   const float T = a.temperature ? a.temperature[row] : a.temperature0;
   const int k = a.top_k ? a.top_k[row] : a.top_k0;
   const float p = a.top_p ? a.top_p[row] : a.top_p0;
   const float mp = a.min_p ? a.min_p[row] : a.min_p0;
-  r.T = T;
+  const int w0 = warp * chunk, w1 = w0 + chunk;
+  r.w0 = w0;
+  r.w1 = w1;
+  r.sub = max(kStep, (chunk / kSubs + kStep - 1) / kStep * kStep);
+  if (threadIdx.x < 4) s.list_count[threadIdx.x] = 0;
 
-  // Slices of whole 16-byte vectors; CTA 0 also takes the entries before the first aligned one.
+  // Slices of whole 16-byte vectors; CTA 0 also takes the entries before the first aligned one, at the end of
+  // its first 8 positions so that vectors land on aligned addresses.
   const int head = min(a.V, int((16 - reinterpret_cast<uintptr_t>(r.src) % 16) % 16 / kSize));
   const int per = ((a.V - head + VEC - 1) / VEC + C - 1) / C * VEC;
   const int vec0 = min(a.V, head + r.rank * per);  // first vector entry of this CTA
-  const int end = min(a.V, vec0 + per);
-  r.begin = r.rank == 0 ? 0 : vec0;
-  r.n = end - r.begin;
-  const int pad = r.rank == 0 ? (8 - head) % 8 : 0;  // vectors land on aligned addresses
-  r.v = reinterpret_cast<float*>(smem_raw + sizeof(Shared)) + pad;
-  r.chunk = (r.n + kWarps * 32 - 1) / (kWarps * 32) * 32;
-  r.w0 = min(r.n, warp * r.chunk);
-  r.w1 = min(r.n, r.w0 + r.chunk);
-
-  uint64_t best = 0;
-  {
-    float bx = -INFINITY;
-    int bi = 0x7fffffff;
-    auto take = [&](float x, int i) {
-      if (x > bx || (x == bx && i < bi)) {
-        bx = x;
-        bi = i;
-      }
-    };
-    auto clean = [](float x) { return x == x ? x + 0.f : -INFINITY; };
-    if (r.rank == 0 && int(threadIdx.x) < head) {
-      const float x = r.logit(threadIdx.x);
-      r.v[threadIdx.x] = x;
-      take(x, threadIdx.x);
-    }
-    const int vecs = (end - vec0) / VEC;
+  const int pad = r.rank == 0 ? (8 - head) % 8 : 0;
+  r.start = r.rank == 0 ? 0 : vec0;
+  r.stop = min(a.V, vec0 + per);
+  r.begin = r.start - pad;
+  float mx = -INFINITY, mn = INFINITY;  // mn: of some finite entries, for the histogram's range
+  if (r.rank == 0 && int(threadIdx.x) < pad + head)
+    r.v[threadIdx.x] = mx = int(threadIdx.x) < pad ? -INFINITY : r.logit(int(threadIdx.x) - pad);
+  // NaN passes through: fmaxf and fminf ignore it.
+  const int vecs = (r.stop - vec0) / VEC;
 #pragma unroll 4
-    for (int g = threadIdx.x; g < vecs; g += kThreads) {
-      const int i = vec0 + g * VEC, j = i - r.begin;
-      const uint4 raw = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(r.src) + int64_t(i) * kSize));
-      float x[VEC];
-      if constexpr (BF16) {
-        const uint32_t q[4] = {raw.x, raw.y, raw.z, raw.w};
+  for (int g = threadIdx.x; g < vecs; g += kThreads) {
+    const int i = vec0 + g * VEC, j = i - r.begin;
+    const uint4 raw = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(r.src) + int64_t(i) * kSize));
+    float x[VEC];
+    if constexpr (BF16) {
+      const uint32_t q[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[2 * e] = clean(bf16_lo(q[e]));
-          x[2 * e + 1] = clean(bf16_hi(q[e]));
-        }
-      } else {
-        x[0] = clean(__uint_as_float(raw.x));
-        x[1] = clean(__uint_as_float(raw.y));
-        x[2] = clean(__uint_as_float(raw.z));
-        x[3] = clean(__uint_as_float(raw.w));
+      for (int e = 0; e < 4; ++e) {
+        x[2 * e] = bf16_lo(q[e]);
+        x[2 * e + 1] = bf16_hi(q[e]);
       }
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) take(x[e], i + e);
-#pragma unroll
-      for (int e = 0; e < VEC; e += 4)
-        *reinterpret_cast<float4*>(&r.v[j + e]) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+    } else {
+      x[0] = __uint_as_float(raw.x);
+      x[1] = __uint_as_float(raw.y);
+      x[2] = __uint_as_float(raw.z);
+      x[3] = __uint_as_float(raw.w);
     }
-    const int rest0 = vec0 + vecs * VEC;
-    if (rest0 + int(threadIdx.x) < end) {
-      const int i = rest0 + threadIdx.x;
-      const float x = r.logit(i);
-      r.v[i - r.begin] = x;
-      take(x, i);
+    if (x[0] > -INFINITY) mn = fminf(mn, x[0]);
+#pragma unroll
+    for (int e = 0; e < VEC; e += 4) {
+      mx = fmaxf(fmaxf(mx, fmaxf(x[e], x[e + 1])), fmaxf(x[e + 2], x[e + 3]));
+      r.quad(j + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
     }
-    best = composite(bx, bi);
   }
-  best = r.block_pick(best, [](uint64_t x, uint64_t y) { return x > y ? x : y; });
+  // The entries after the last whole vector, then the padding.
+  for (int j = vec0 + vecs * VEC - r.begin + int(threadIdx.x); j < chunk * kWarps; j += kThreads) {
+    const float x = r.begin + j < r.stop ? r.logit(r.begin + j) : -INFINITY;
+    r.v[j] = x;
+    mx = fmaxf(mx, x);
+  }
   {
-    const uint64_t(*x)[kMaxCluster] = r.exchange(best);
-    for (int q = 0; q < C; ++q) best = max(best, x[0][q]);
+    const uint32_t top = __reduce_max_sync(0xffffffffu, order_key(mx + 0.f));
+    const uint32_t low = __reduce_max_sync(0xffffffffu, ~order_key(mn));
+    if (lane == 0) {
+      s.red32[0][warp] = top;
+      s.red32[1][warp] = low;
+    }
+    __syncthreads();
+    const uint64_t(*x)[kMaxCluster] = r.exchange(__reduce_max_sync(0xffffffffu, s.red32[0][lane % kWarps]),
+                                                 __reduce_max_sync(0xffffffffu, s.red32[1][lane % kWarps]));
+    uint64_t t = 0, l = 0;
+    for (int q = 0; q < C; ++q) {
+      t = max(t, x[0][q]);
+      l = max(l, x[1][q]);
+    }
+    mx = key_value(uint32_t(t));
+    mn = key_value(~uint32_t(l));
   }
-  r.mx = key_value(uint32_t(best >> 32));
-  r.first = int(~uint32_t(best));
-  if (r.mx == -INFINITY || !(T > 0.f)) {  // the same in all CTAs of the row; no remote access follows
+  r.mx = mx;
+  if (mx == -INFINITY) {  // the same in all CTAs of the row; no remote access follows
     if (r.rank == 0 && threadIdx.x == 0) {
-      a.tokens[row] = r.mx == -INFINITY ? -1 : r.first;
-      a.logprobs[row] = r.mx == -INFINITY ? -INFINITY : 0.f;
+      a.tokens[row] = -1;
+      a.logprobs[row] = -INFINITY;
     }
     return;
   }
-  const int w0 = r.w0, w1 = r.w1;
-  const bool cut_k = k > 0 && k < a.V, cut_p = p < 1.f;
-  uint64_t cut = 0;  // entries of composite >= cut are kept
-  if (cut_k || cut_p) {
-    for (int j = w0 + lane; j < w1; j += 32) r.v[j] = r.dist(r.v[j]);
-    auto by_distance = [&](int j, int& b, float& w) {
-      const float d = r.v[j];
-      if (!(d > -kSpan)) return false;
-      b = Row<BF16>::bin(d);
-      w = Row<BF16>::weight(d);
-      return true;
-    };
-    r.histogram(by_distance, cut_p);
-    bool rebuilt = false;
-    uint64_t through = r.total_mass;
-    typename Row<BF16>::Goal g;
-    if (cut_k && uint64_t(k) < r.total_count) {
-      g.by_mass = false;
-      g.k = k;
-      g.want = 0.;
-      cut = r.find_cut(g, 0, through, rebuilt);
+  if (!(T > 0.f) || k == 1 || p <= 0.f || mp > 1.f) {  // only the best entry: the first of the equal ones
+    uint64_t first = kNothing;
+    r.sweep(w0, w1, [&](int j, const float (&x)[4]) {
+#pragma unroll
+      for (int e = 3; e >= 0; --e)
+        if (x[e] == mx) first = min(first, uint64_t(r.begin + j + e));
+    });
+    first = r.block_min(first);
+    const uint64_t(*x)[kMaxCluster] = r.exchange(first);
+    for (int q = 0; q < C; ++q) first = min(first, x[0][q]);
+    if (r.rank == 0 && threadIdx.x == 0) {
+      a.tokens[row] = int64_t(first);
+      a.logprobs[row] = 0.f;
     }
+    return;
+  }
+  float base = mx;
+  r.T = T;
+  r.scale = 1.f;
+  if (!(T > 0x1p-40f && T < 0x1p40f && mx < INFINITY)) {
+    // An extreme temperature (or infinite logits): differences and T by a power of two, T towards 1.
+    r.scale = T < INFINITY ? ldexpf(1.f, min(126, max(-126, -ilogbf(T)))) : 0.f;
+    r.T = T < INFINITY ? T * r.scale : 1.f;
+    base = 0.f;
+    for (int j = w0 + lane; j < w1; j += 32) {
+      const float x = r.v[j];
+      r.v[j] = x == mx ? 0.f : x > -INFINITY ? (x - mx) * r.scale : -INFINITY;
+    }
+    __syncwarp();
+  }
+  r.inv = 1.f / r.T;
+  const bool cut_k = k > 0 && k < a.V, cut_p = p < 1.f;
+  uint64_t cut = 0;     // entries of composite >= cut are kept
+  bool summed = false;  // s.sub holds the kept masses
+  if (cut_k || cut_p) {
+    // Histogram of d over its range: bin = -d * bins rounded by the addition of 2^23.
+    const float range = fminf(kSpan, fmaxf(0x1p-20f, -r.dist(mn)));
+    const float bins = (kBins - 1) / range;
+    auto bin_of = [&](float d) { return min(kBins - 1, __float_as_int(fmaf(-d, bins, 8388608.f)) - 0x4b000000); };
+    r.clear_histogram();
+    if (cut_p)
+      r.first_sweep(w0, w1, base, [&](int, const float (&d)[4]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint64_t m = mass_of(R::weight(d[e]));
+          if (m) {
+            const int b = bin_of(d[e]);
+            if (cut_k) atomicAdd(&s.cnt[b], 1u);
+            r.add_mass(b, m);
+          }
+        }
+      });
+    else
+      r.first_sweep(w0, w1, base, [&](int, const float (&d)[4]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (d[e] > -kSpan) atomicAdd(&s.cnt[bin_of(d[e])], 1u);
+      });
+    r.merge();
+    auto rebuild = [&]() {  // after the histogram's memory was used
+      r.histogram([&](int j, int& b, float& w) {
+        const float d = r.v[j];
+        if (!(d > -kSpan)) return false;
+        b = bin_of(d);
+        w = R::weight(d);
+        return true;
+      });
+    };
+    uint64_t through = r.total_mass;  // mass left by top-k
+    typename R::Goal gk{false, uint64_t(k), 0.}, gp{true, 0, 0.};
+    typename R::Cut ck{-1, 0, 0, 0, 0}, cp{-1, 0, 0, 0, 0};
+    if (cut_k && uint64_t(k) < r.total_count) ck = r.find_bin(gk);
+    bool k_done = ck.bin < 0;  // fewer entries with mass than k: no cut
+    auto slow = [&](const typename R::Cut& c, const typename R::Goal& g, uint64_t& t) {
+      return r.find_cut(
+          [&](float x) {
+            const float d = r.dist(x);
+            return d > -kSpan && bin_of(d) == c.bin;
+          },
+          c, g, t);
+    };
+    typename R::Cut cq = cp;
     if (cut_p) {
-      g.by_mass = true;
-      g.k = 0;
-      g.want = double(p) * double(through);
-      if (!(g.want > 0.)) {
-        cut = best;
+      // Bounds of the mass left by top-k bound the bins in which top-p can cut.
+      const uint64_t low = k_done ? through : ck.mass, high = k_done ? through : ck.mass + ck.bin_mass;
+      gp.want = double(p) * double(low);
+      if (low > 0) cp = r.find_bin(gp);
+      else cp.bin = 0;  // top-k cuts in the first bin that has entries
+      cq = cp;
+      if (high != low) {
+        gp.want = double(p) * double(high);
+        cq = r.find_bin(gp);
+      }
+    }
+    if (cut_p || !k_done) {
+      // One pass: entries before the first cut bin are kept for certain, those of the cut bins are listed.
+      const int kb = k_done ? -1 : ck.bin, p0 = cut_p ? cp.bin : kBins, p1 = cut_p ? cq.bin : -1;
+      const int sure = cut_p ? p0 : kb;
+      auto group = [&](int b) { return (b == kb ? kInK : 0ull) | (b >= p0 && b <= p1 ? kInP : 0ull); };
+      const int n = r.gather(
+          [&](float d, bool& want) -> uint64_t {
+            const int b = bin_of(d);
+            if (b < sure) {
+              const float w = R::weight(d);
+              return mass_of(w < mp ? 0.f : w);
+            }
+            want = (b == kb || (b >= p0 && b <= p1)) && d > -kSpan;
+            return 0;
+          },
+          [&](float x) { return group(bin_of(r.dist(x))); });
+      if (n <= kList) {
+        cut = r.rank_list(n, !k_done, gk, ck, cut_p, p, cp, through);
+        // The listed entries of this CTA that are kept after all.
+        for (int e = threadIdx.x; e < int(s.own_count); e += kThreads) {
+          const uint64_t c = s.list[s.own_base + e].x;
+          if (c >= cut) {
+            const float w = R::weight(r.dist(key_value(uint32_t(c >> 32))));
+            const int j = s.own[e], part = j / chunk * kSubs + j % chunk / r.sub;
+            if (!(w < mp)) atomicAdd(reinterpret_cast<unsigned long long*>(&s.sub[part]), mass_of(w));
+          }
+        }
+        __syncthreads();
+        summed = true;
       } else {
-        if (rebuilt) r.histogram(by_distance, true);
-        uint64_t unused;
-        cut = max(cut, r.find_cut(g, cut, unused, rebuilt));
+        if (!k_done) {
+          cut = slow(ck, gk, through);
+          if (cut_p) rebuild();
+        }
+        if (cut_p) {
+          gp.want = double(p) * double(through);
+          cp = r.find_bin(gp);
+          uint64_t unused;
+          cut = max(cut, slow(cp, gp, unused));
+        }
       }
     }
   }
-  // Weights of the kept entries, their mass, then the draw.
-  cut = min(cut, best);
-  const float cut_x = key_value(uint32_t(cut >> 32));
-  const float cut_d = cut == 0 ? -INFINITY : r.dist(cut_x);
-  uint32_t sh = 0, sl = 0;
-  const bool filtered = cut_k || cut_p;
-  for (int j = w0 + lane; j < w1; j += 32) {
-    float d = r.v[j];
-    if (!filtered) d = r.dist(d);
-    float w = 0.f;
-    if (d > -kSpan && d >= cut_d) {
-      w = Row<BF16>::weight(d);
-      const int i = r.begin + j;
-      if (w < mp) w = 0.f;
-      else if (d == cut_d && cut != 0 && composite(r.logit(i), i) < cut) w = 0.f;
-      if (i == r.first) w = 1.f;
-      uint32_t h, l;
-      mass_halves(w, h, l);
-      sh += h;
-      sl += l;
-    }
-    r.v[j] = w;
-  }
-  uint64_t mass = warp_sum64((uint64_t(sh) << 18) + sl);  // at most 32 halves of 18 bits each
-  if (lane == 0) s.wsum[warp] = mass;
-  __syncthreads();
+  // Masses of the kept entries, then the draw.  (A cut always keeps the first entry of its bin.)  d decides
+  // except at the cut itself, and among entries too close to the best one to be told apart by it.
+  const float cut_d = cut == 0 ? -INFINITY : r.dist(key_value(uint32_t(cut >> 32)));
+  const float cut_low = fminf(cut_d, -kTiny), cut_high = cut_d < -kTiny ? cut_d : 0.f;
+  auto kept_weight = [&](float d, int j) -> float {
+    const float w = R::weight(d);
+    if (cut == 0) return w < mp ? 0.f : w;
+    if (!(d >= cut_low) || w < mp || (d <= cut_high && composite(r.at(j), r.begin + j) < cut)) return 0.f;
+    return w;
+  };
   uint64_t mine = 0;
+  if (summed) {
+    if (lane < kSubs) mine = s.sub[warp * kSubs + lane];
+    mine = warp_sum64(mine);
+  } else {
+    for (int i = 0; i < kSubs; ++i) {
+      uint64_t m = 0;
+      const int j0 = w0 + i * r.sub, j1 = min(w1, j0 + r.sub);
+      if (cut_k || cut_p)
+        r.sweep(j0, j1, [&](int j, const float (&d)[4]) {
 #pragma unroll
-  for (int i = 0; i < kWarps; ++i) mine += s.wsum[i];
+          for (int e = 0; e < 4; ++e) m += mass_of(kept_weight(d[e], j + e));
+        });
+      else
+        r.first_sweep(j0, j1, base, [&](int, const float (&d)[4]) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float w = R::weight(d[e]);
+            m += mass_of(w < mp ? 0.f : w);
+          }
+        });
+      m = warp_sum64(m);
+      if (lane == 0) s.sub[warp * kSubs + i] = m;
+      mine += m;
+    }
+  }
+  mine = r.block_sum(lane == 0 ? mine : 0);
   const uint64_t(*x)[kMaxCluster] = r.exchange(mine);
   uint64_t total = 0, before = 0;
   for (int q = 0; q < C; ++q) {
@@ -622,29 +837,68 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
   }
   uint64_t target = uint64_t(fmax(0., floor(double(a.u[row]) * double(total))));
   target = min(target, total - 1);
-  if (target < before || target >= before + mine) return;
-  for (int i = 0; i < warp; ++i) before += s.wsum[i];
-  if (target < before || target >= before + mass) return;
-  const int j = r.select_in_warp([&](int e) { return mass_of(r.v[e]); }, target, before);
-  if (lane == 0) {
-    const int i = r.begin + j;
-    a.tokens[row] = i;
-    a.logprobs[row] = float(double(r.dist(r.logit(i))) - log(double(total) / double(kFixed)));
+  if (warp != 0 || target < before || target >= before + mine) return;
+  // Warp 0 of the CTA that holds the token: the part, the step of 128, the entry.
+  constexpr int kPer = kWarps * kSubs / 32;
+  uint64_t m[kPer], sum = 0;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) sum += m[e] = s.sub[kPer * lane + e];
+  uint64_t c = before + warp_inclusive64(sum) - sum;
+  int part = -1;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) {
+    if (target >= c && target < c + m[e]) {
+      part = kPer * lane + e;
+      before = c;
+    }
+    c += m[e];
+  }
+  const int owner = __ffs(__ballot_sync(0xffffffffu, part >= 0)) - 1;
+  part = __shfl_sync(0xffffffffu, part, owner);
+  before = __shfl_sync(0xffffffffu, before, owner);
+  const int j0 = part / kSubs * chunk + part % kSubs * r.sub;
+  for (int j = j0 + 4 * lane;; j += kStep) {
+    const float4 f = r.quad(j);
+    const float d[4] = {f.x, f.y, f.z, f.w};
+    uint64_t q[4], sum4 = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum4 += q[e] = mass_of(kept_weight(d[e], j + e));
+    const uint64_t inc = warp_inclusive64(sum4);
+    const uint64_t step = __shfl_sync(0xffffffffu, inc, 31);
+    if (target >= before + step && j - 4 * lane + kStep < j0 + r.sub) {
+      before += step;
+      continue;
+    }
+    uint64_t b = before + inc - sum4;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (target >= b && target < b + q[e]) {
+        a.tokens[row] = r.begin + j + e;
+        // log(total / 2^36) through what exceeds 1 (the best entry's mass is 2^36), exact before its rounding.
+        a.logprobs[row] = d[e] - log1pf(float(total - (1ull << 36)) / kFixed);
+      }
+      b += q[e];
+    }
+    break;
   }
 }
 
 }  // namespace
 
-int sample_max_vocabulary() { return kMaxCluster * (kMaxSlice - 16); }
+// Positions of a CTA: whole vectors of 8, plus 8 of padding in the first.
+static int slice_positions(int V, int C) { return ((V + 7) / 8 + C - 1) / C * 8 + 16; }
+
+int sample_max_vocabulary() { return kMaxCluster * (kSlice - 32); }
 
 void launch_sample_tokens(const SampleArgs& a, cudaStream_t stream) {
   if (a.R == 0) return;
   if (a.V < 1 || a.V > sample_max_vocabulary()) throw std::invalid_argument("sample_tokens: vocabulary size");
-  auto slice = [&](int c) { return ((a.V + 7) / 8 + c - 1) / c * 8 + 8; };
   int C = 1;
-  while (C < kMaxCluster && slice(C) > 8192 + 8) C *= 2;
-  const int cap = slice(C) + 8;
-  const size_t smem = sizeof(Shared) + size_t(cap) * 4;
+  while (slice_positions(a.V, C) > kSlice) C *= 2;
+  // Few rows: more CTAs for each while two fit every SM.
+  while (C < kMaxCluster && slice_positions(a.V, C) > 4096 && int64_t(a.R) * C * 2 <= 2 * sm_count()) C *= 2;
+  const int chunk = (slice_positions(a.V, C) + kWarps * kStep - 1) / (kWarps * kStep) * kStep;
+  const size_t smem = sizeof(Shared) + size_t(chunk) * kWarps * 4;
   auto kernel = a.bf16 ? sample_kernel<true> : sample_kernel<false>;
   cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)), "sample_tokens smem");
   cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "sample_tokens cluster");
@@ -662,7 +916,7 @@ void launch_sample_tokens(const SampleArgs& a, cudaStream_t stream) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl_flag() ? 2 : 1;
-  cuda_check(cudaLaunchKernelEx(&cfg, kernel, a, C), "sample_tokens launch");
+  cuda_check(cudaLaunchKernelEx(&cfg, kernel, a, C, chunk), "sample_tokens launch");
 }
 
 }  // namespace b200
