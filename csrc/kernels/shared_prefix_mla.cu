@@ -29,11 +29,12 @@
 //    thread and completing on CTA 0's barriers.  Tail tiles are loaded by
 //    cp.async instead, which zero-fills the rows past the visible ones: memory
 //    there may hold NaN, and 0 * NaN in PV would spread it.
-//  * Softmax: 8 warps; the four threads of a row (TMEM lanes r and r + 64, two
-//    warpgroups) take 16 keys of a tile each and agree on the maximum through
-//    shared memory.  The running maximum is raised only when it grows by more
-//    than 2^8 (O is then rescaled), P is rounded to BF16 (what the MMA takes),
-//    its sum is kept unrounded in FP32.
+//  * Softmax: two warpgroups take the tiles in turn; the two threads of a row
+//    (TMEM lanes r and r + 64) hold 32 keys of a tile each and agree on the
+//    maximum through shared memory.  The running maximum passes from tile to
+//    tile; it is raised only when it grows by more than 2^8 (O is then
+//    rescaled).  P is rounded to BF16 (what the MMA takes), its sum is kept
+//    unrounded in FP32.
 //
 // Row tiles rarely fill the SM pairs evenly, so the key ranges of the tiles
 // that do not make up whole waves are cut into equal shares, one per pair; a
@@ -59,20 +60,21 @@ constexpr int BM = 128;                   // rows per unit (pair)
 constexpr int MC = 64;                    // rows per CTA
 constexpr int BN = 64;                    // keys per tile (pair)
 constexpr int BNC = 32;                   // keys per tile per CTA (QK's B split)
-constexpr int STAGES = 3;                 // record ring (a stage is held from its load to the tile's PV)
+constexpr int STAGES = 4;                 // record ring (a stage is held from its load to the tile's PV)
+constexpr int PBUF = 2;                   // P buffers
 constexpr int SBUF = 4;                   // S buffers in TMEM
 constexpr int kChunks = D / 64;
 constexpr int kQChunkBytes = MC * 128;
 constexpr int kKeyChunkBytes = BNC * 128;
-constexpr int kPBytes = MC * 128;         // 64 rows x 64 keys BF16
+constexpr int kPBytes = MC * 64;          // half of P: 64 rows x 32 keys BF16
 constexpr int kSoftmaxWarps = 8;          // warps 0-7
 constexpr int kSoftmaxThreads = kSoftmaxWarps * 32;
 constexpr int kOwnWarp0 = 8;              // warps 8, 9: Q + records
 constexpr int kOwnWarps = 2;
-constexpr int kPvWarp0 = 10;              // warps 10, 11: peer keys' value dims
-constexpr int kPvWarps = 2;
-constexpr int kMmaWarp = 12;
-constexpr int kThreads = 13 * 32;
+constexpr int kPvWarp0 = 10;              // warp 10: peer keys' value dims
+constexpr int kPvWarps = 1;
+constexpr int kMmaWarp = 11;
+constexpr int kThreads = 12 * 32;
 constexpr uint32_t kQBytes = kChunks * kQChunkBytes;
 constexpr uint32_t kOwnBytes = kChunks * kKeyChunkBytes;  // records of a CTA's 32 keys
 constexpr uint32_t kPvBytes = 4 * kKeyChunkBytes;         // the peer's 32 keys x 256 value dims
@@ -81,18 +83,20 @@ constexpr uint32_t kTmemS = 256;                          // O half v at [128v, 
 
 constexpr int kOffQ = 0;                                            // [9][8 KB]
 constexpr int kOffOwn = kOffQ + kChunks * kQChunkBytes;             // [STAGES][9][4 KB]
-constexpr int kOffP = kOffOwn + STAGES * kChunks * kKeyChunkBytes;  // [2][8 KB]
-constexpr int kOffSmall = kOffP + 2 * kPBytes;
+constexpr int kOffP = kOffOwn + STAGES * kChunks * kKeyChunkBytes;  // [PBUF][4 KB]
+constexpr int kOffSmall = kOffP + PBUF * kPBytes;
 
 struct Small {
-  float red[2][kSoftmaxThreads];  // tile maxima of a row's four threads; in the end the denominators
+  float red[2][kSoftmaxThreads];  // tile maxima of a row's two threads (double buffered); in the end the denominators
+  float m_run[2][MC];             // running maximum after a tile (by tile parity)
+  uint64_t m_ready[2];            // the tile's running maximum is in m_run
   uint64_t q_full;                // CTA 0: Q rows of both CTAs
   uint64_t own_full[STAGES];      // CTA 0: records of the tile
   uint64_t pv_full[STAGES];       // CTA 0: peer keys' value dims
   uint64_t pv_done[STAGES];       // PV of the tile done (commit): stage and P buffer free
   uint64_t s_full[SBUF];          // QK of the tile done (commit)
   uint64_t s_empty[SBUF];         // CTA 0: both CTAs' softmax warps read S
-  uint64_t p_full[2];             // CTA 0: both CTAs' softmax warps wrote P
+  uint64_t p_full[PBUF];           // CTA 0: both CTAs' softmax warps wrote P
   uint64_t o_full;                // last PV done (commit)
   uint32_t tmem_base;
   int abort_flag;
@@ -146,6 +150,17 @@ __device__ __forceinline__ void mma_pair_ss(uint32_t d_tmem, uint64_t a_desc, ui
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// K-major operand tile of 64-byte rows with the 64-byte swizzle: 16-byte units
+// XORed with address bits 7-8, 8-row groups 512 bytes apart.
+__device__ __forceinline__ uint64_t umma_desc_sw64(uint32_t addr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((addr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>(1u) << 16;         // LBO (unused for swizzled K-major)
+  d |= static_cast<uint64_t>(512u >> 4) << 32;  // SBO
+  d |= static_cast<uint64_t>(1u) << 46;         // version (sm100)
+  d |= static_cast<uint64_t>(4u) << 61;         // SWIZZLE_64B
+  return d;
+}
 // Arrive on the mbarrier at shared::cluster address `bar` once the pair's previously issued MMAs complete.
 __device__ __forceinline__ void commit_pair(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
@@ -162,13 +177,14 @@ __device__ __forceinline__ bool mbar_test_cluster(uint64_t* bar, uint32_t parity
   return ok != 0;
 }
 // Every thread of the barrier gets the OR of the predicates.
-__device__ __forceinline__ bool bar_red_or(uint32_t id, uint32_t nthreads, bool pred) {
+template <int ID>
+__device__ __forceinline__ bool bar_red_or(uint32_t nthreads, bool pred) {
   uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
       "bar.red.or.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
-      : "r"(uint32_t(pred)), "r"(id), "r"(nthreads)
+      : "r"(uint32_t(pred)), "n"(ID), "r"(nthreads)
       : "memory");
   return r != 0;
 }
@@ -272,7 +288,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto own_chunk = [&](int st, int j) { return sbase + kOffOwn + (st * kChunks + j) * kKeyChunkBytes; };
   // PV's B operand (value dims, MN-major) of key half kh and value half v.
   auto pv_region = [&](int st, int kh, int v) { return own_chunk(st, 4 * v + 2 * kh); };
-  const uint32_t p_buf[2] = {sbase + kOffP, sbase + kOffP + kPBytes};
+  // P of tile i in two K halves (64-byte swizzle): keys [0, 32) take the tile's record chunk of the RoPE dims,
+  // which only QK needed, keys [32, 64) a buffer of their own.
+  auto p_half = [&](int i, int kh) {
+    return kh == 0 ? own_chunk(i % STAGES, kChunks - 1) : sbase + kOffP + (i % PBUF) * kPBytes;
+  };
   // Tile i: first key row of its source (prefix or tail) and how many of its 64 keys are visible.
   auto tile_key0 = [&](int i) { return (i < w.np ? w.p0 + i : w.t0 + i - w.np) * BN; };
   auto tile_valid = [&](int i) { return min(BN, (i < w.np ? a.P : w.seen) - tile_key0(i)); };
@@ -286,9 +306,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < SBUF; ++i) {
       mbar_init(&s.s_full[i], 1);
-      mbar_init(&s.s_empty[i], 2 * kSoftmaxWarps);
+      mbar_init(&s.s_empty[i], kSoftmaxWarps);  // a tile is read by 4 warps of each CTA
     }
-    for (int i = 0; i < 2; ++i) mbar_init(&s.p_full[i], 2 * kSoftmaxWarps);
+    for (int i = 0; i < PBUF; ++i) mbar_init(&s.p_full[i], kSoftmaxWarps);
+    for (int i = 0; i < 2; ++i) mbar_init(&s.m_ready[i], kSoftmaxWarps / 2);
     mbar_init(&s.o_full, 1);
     s.abort_flag = 0;
     fence_barrier_init();
@@ -419,17 +440,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         commit_pair(peer(&s.s_full[b]));
       };
       auto issue_pv = [&](int i) {
-        const int st = i % STAGES, b = i & 1;
+        const int st = i % STAGES;
         fence_proxy_async();
         tc_fence_after();
-        const uint64_t pdesc = umma_desc_sw128(p_buf[b]);
 #pragma unroll
         for (int v = 0; v < 2; ++v) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             // Keys [16k, +16): key half k / 2, row offset 16 (k % 2) in its region.
             const uint64_t vdesc = umma_desc_sw128_mn(pv_region(st, k >> 1, v) + (k & 1) * 16 * 128, kKeyChunkBytes);
-            mma_pair_ss(tmem + v * 128, pdesc + ((k * 32) >> 4), vdesc, idesc_pv, (i > 0 || k > 0) ? 1u : 0u);
+            const uint64_t pdesc = umma_desc_sw64(p_half(i, k >> 1) + (k & 1) * 32);
+            mma_pair_ss(tmem + v * 128, pdesc, vdesc, idesc_pv, (i > 0 || k > 0) ? 1u : 0u);
           }
         }
         commit_pair(smem_u32(&s.pv_done[st]));
@@ -444,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           issue_qk(nq++);
           progressed = true;
         }
-        if (np < nq && mbar_test_cluster(&s.p_full[np & 1], (np >> 1) & 1) &&
+        if (np < nq && mbar_test_cluster(&s.p_full[np % PBUF], (np / PBUF) & 1) &&
             mbar_test_cluster(&s.pv_full[np % STAGES], (np / STAGES) & 1)) {
           issue_pv(np++);
           progressed = true;
@@ -468,94 +489,107 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp < kSoftmaxWarps) {
     // ------------------------------------------------------------ softmax
-    // The threads leave the tile loop together: a failed wait is carried to
-    // the next bar.red.or, which every thread reaches.  TMEM loads and stores
-    // run only under warp-uniform conditions.
+    // The two warpgroups take the tiles in turn.  The threads of one leave its
+    // tile loop together: a failed wait is carried to the next bar.red.or,
+    // which every thread of the warpgroup reaches.  TMEM loads and stores run
+    // only under warp-uniform conditions.
     const int tt = threadIdx.x;
-    const int wg = tt >> 7;             // warpgroup: which 16 of the lane's 32 S columns
+    const int wg = tt >> 7;
     const int hrow = tt & 63;           // row within the CTA
     const int kh = (tt >> 6) & 1;       // key half (CTA kh's keys)
     const uint32_t lane_addr = uint32_t((warp & 3) * 32) << 16;
-    const int col0 = 32 * kh + 16 * wg; // first key of this thread in a tile
-    float m_used = -INFINITY, l = 0.f;
+    float m_used = -INFINITY, l = 0.f;  // l is relative to m_used
     bool pending_fail = false;
     bool failed = false;
-    for (int i = 0; i < ntiles; ++i) {
+    for (int i = wg; i < ntiles; i += 2) {
       const int b = i % SBUF;
-      const int pb = i & 1;
-      const int valid = tile_valid(i) - col0;  // this thread's keys j < valid count
+      const int rb = (i >> 1) & 1;
+      const int valid = tile_valid(i) - BNC * kh;  // this thread's keys j < valid count
       bool got = __all_sync(0xffffffffu, mbar_wait(&s.s_full[b], (i / SBUF) & 1, err, kErrTimeoutTmemFull, abort_flag));
-      uint32_t r[16];
+      uint32_t r[32];
       if (got) {
         tc_fence_after();
-        tmem_ld16(tmem + lane_addr + kTmemS + b * (BN / 2) + 16 * wg, r);
+        tmem_ld32(tmem + lane_addr + kTmemS + b * (BN / 2), r);
         tmem_wait_ld();
-        tmem_regs_ready16(r);
+        tmem_regs_ready(r);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) arrive_leader(&s.s_empty[b]);
       } else {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) r[j] = 0u;
+        for (int j = 0; j < 32; ++j) r[j] = 0u;
       }
-      if (valid < 16) {
+      if (valid < BNC) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
+        for (int j = 0; j < 32; ++j)
           if (j >= valid) r[j] = 0xff800000u;  // -inf: weight 0
       }
-      float mx[4];
+      float mx[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        mx[j] = fmaxf(fmaxf(__uint_as_float(r[j]), __uint_as_float(r[j + 4])),
-                      fmaxf(__uint_as_float(r[j + 8]), __uint_as_float(r[j + 12])));
+      for (int j = 0; j < 8; ++j)
+        mx[j] = fmaxf(fmaxf(__uint_as_float(r[j]), __uint_as_float(r[j + 8])),
+                      fmaxf(__uint_as_float(r[j + 16]), __uint_as_float(r[j + 24])));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) mx[j] = fmaxf(mx[j], mx[j + 4]);
       float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2;  // the scale is positive
-      s.red[pb][tt] = mt;
-      if (bar_red_or(1, kSoftmaxThreads, !got || pending_fail)) {
+      s.red[rb][tt] = mt;
+      const bool fail = wg == 0 ? bar_red_or<1>(kSoftmaxThreads / 2, !got || pending_fail)
+                                : bar_red_or<2>(kSoftmaxThreads / 2, !got || pending_fail);
+      if (fail) {
         failed = true;
         break;
       }
-      mt = fmaxf(fmaxf(mt, s.red[pb][tt ^ 64]), fmaxf(s.red[pb][tt ^ 128], s.red[pb][tt ^ 192]));
-      bool rescale = false;
-      float alpha = 1.f;
-      if (m_used == -INFINITY) {
-        m_used = mt;
-      } else if (mt > m_used + kRescaleThreshold) {
-        alpha = exp2f(m_used - mt);
-        l *= alpha;
-        m_used = mt;
-        rescale = true;
+      mt = fmaxf(mt, s.red[rb][tt ^ 64]);
+      // The running maximum after tile i - 1 comes from the other warpgroup, which has published it long
+      // before it is done with that tile.
+      float m_prev = -INFINITY;
+      bool clear = true;
+      if (i > 0) {
+        clear = __all_sync(0xffffffffu, mbar_wait(&s.m_ready[(i - 1) & 1], ((i - 1) >> 1) & 1, err, kErrTimeoutGeneric,
+                                                  abort_flag));
+        m_prev = s.m_run[(i - 1) & 1][hrow];
       }
-      const float mbase = m_used == -INFINITY ? 0.f : m_used;
-      uint32_t pk[8];
-      float ps[2] = {0.f, 0.f};
+      const float m = (m_prev == -INFINITY || mt > m_prev + kRescaleThreshold) ? mt : m_prev;
+      if (kh == 0) s.m_run[i & 1][hrow] = m;  // both threads of the row hold the same value
+      // (lanes r and r + 64 are different warps: each warp's arrival follows its own writes)
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.m_ready[i & 1]);
+      const bool rescale = i > 0 && m_prev != -INFINITY && m != m_prev;
+      const float alpha = rescale ? exp2f(m_prev - m) : 1.f;
+      if (m != m_used) {
+        l = m_used == -INFINITY ? 0.f : l * exp2f(m_used - m);
+        m_used = m;
+      }
+      const float mbase = m == -INFINITY ? 0.f : m;
+      uint32_t pk[16];
+      float ps[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < 16; ++j) {
         const float x = ex2_approx(fmaf(__uint_as_float(r[2 * j]), scale_log2, -mbase));
         const float y = ex2_approx(fmaf(__uint_as_float(r[2 * j + 1]), scale_log2, -mbase));
-        ps[j & 1] += x + y;
+        ps[j & 3] += x + y;
         pk[j] = pack_bf16(x, y);
       }
-      l += ps[0] + ps[1];
-      // P(i) reuses the buffer of P(i - 2): wait for PV(i - 2).
-      bool clear = true;
-      if (i >= 2)
-        clear = __all_sync(0xffffffffu, mbar_wait(&s.pv_done[(i - 2) % STAGES], ((i - 2) / STAGES) & 1, err,
+      l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+      // P(i) reuses the buffer of P(i - PBUF): wait for its PV.
+      if (clear && i >= PBUF)
+        clear = __all_sync(0xffffffffu, mbar_wait(&s.pv_done[(i - PBUF) % STAGES], ((i - PBUF) / STAGES) & 1, err,
                                                   kErrTimeoutTmemEmpty, abort_flag));
-      if (clear && i >= 1 && __any_sync(0xffffffffu, rescale)) {
+      if (clear && __any_sync(0xffffffffu, rescale)) {
         // O is touched only after PV(i - 1), the last MMA adding into it, is done.
         clear = __all_sync(0xffffffffu, mbar_wait(&s.pv_done[(i - 1) % STAGES], ((i - 1) / STAGES) & 1, err,
                                                   kErrTimeoutTmemEmpty, abort_flag));
         if (clear) {
           tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
+          for (int c = 0; c < 8; ++c) {
             uint32_t o[32];
-            tmem_ld32(tmem + lane_addr + wg * 128 + c * 32, o);
+            tmem_ld32(tmem + lane_addr + c * 32, o);
             tmem_wait_ld();
             tmem_regs_ready(o);
 #pragma unroll
             for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
-            tmem_st32(tmem + lane_addr + wg * 128 + c * 32, o);
+            tmem_st32(tmem + lane_addr + c * 32, o);
           }
           tmem_wait_st();
         }
@@ -564,11 +598,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         pending_fail = true;
         continue;
       }
-      // P row hrow, keys [col0, +16): two 16-byte units of the swizzled 128-byte row.
+      // P row hrow, keys [32 kh, +32): the four 16-byte units of a swizzled 64-byte row.
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int u = (col0 >> 3) + j;
-        const uint32_t dst = p_buf[pb] + hrow * 128 + ((u ^ (hrow & 7)) << 4);
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t dst = p_half(i, kh) + hrow * 64 + ((j ^ ((hrow >> 1) & 3)) << 4);
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(pk[4 * j]), "r"(pk[4 * j + 1]),
                      "r"(pk[4 * j + 2]), "r"(pk[4 * j + 3])
                      : "memory");
@@ -576,18 +609,26 @@ __global__ void __launch_bounds__(kThreads, 1)
       fence_proxy_async();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) arrive_leader(&s.p_full[pb]);
+      if (lane == 0) arrive_leader(&s.p_full[i % PBUF]);
     }
-    // ---- epilogue: O / l over the four threads of each row.  Every read of
-    // red[ntiles & 1] (tile ntiles - 2) happened before the last tile's
-    // barrier, so the buffer is free for the denominators.
-    float* lsum = s.red[ntiles & 1];
+    // ---- epilogue: O / l over the four threads of each row, relative to the
+    // last tile's maximum.  The denominators take the `red` buffer that the
+    // warpgroup's last tile did not use (read before that tile's barrier).
+    const int mine = ntiles > wg ? (ntiles - 1 - wg) / 2 : 1;          // index of this warpgroup's last tile
+    const int theirs = ntiles > 1 - wg ? (ntiles - 1 - (1 - wg)) / 2 : 1;
+    float* lsum = s.red[(mine & 1) ^ 1];
+    const float* lsum_other = s.red[(theirs & 1) ^ 1];
     lsum[tt] = l;
-    const bool any_fail = bar_red_or(1, kSoftmaxThreads, failed || pending_fail);
-    const float lt = (l + lsum[tt ^ 64]) + (lsum[tt ^ 128] + lsum[tt ^ 192]);
+    const bool any_fail = bar_red_or<3>(kSoftmaxThreads, failed || pending_fail);
+    const float l_own = l + lsum[tt ^ 64], l_other = lsum_other[tt ^ 128] + lsum_other[tt ^ 192];
+    // m_run holds the maxima after each warpgroup's last tile.
+    const float m_last = ntiles > 0 ? s.m_run[(ntiles - 1) & 1][hrow] : -INFINITY;
+    const float m_other = ntiles > (wg ^ 1) ? s.m_run[wg ^ 1][hrow] : -INFINITY;
+    const float lt = (m_used == -INFINITY ? l_own : l_own * exp2f(m_used - m_last)) +
+                     (m_other == -INFINITY ? l_other : l_other * exp2f(m_other - m_last));
     // A row without visible keys has sum 0; NaN scores stay NaN.
     const float inv = lt == 0.f ? 0.f : 1.f / lt;
-    const float lse = lt == 0.f ? -INFINITY : (m_used == -INFINITY ? 0.f : m_used) * 0.69314718055994531f + logf(lt);
+    const float lse = lt == 0.f ? -INFINITY : (m_last == -INFINITY ? 0.f : m_last) * 0.69314718055994531f + logf(lt);
     const bool have_o = !any_fail && ntiles > 0 &&
                         __all_sync(0xffffffffu, mbar_wait(&s.o_full, 0, err, kErrTimeoutTmemFull, abort_flag));
     if (have_o) tc_fence_after();
