@@ -69,11 +69,12 @@ constexpr int kKeyChunkBytes = BNC * 128;
 constexpr int kPBytes = MC * 64;          // half of P: 64 rows x 32 keys BF16
 constexpr int kSoftmaxWarps = 8;          // warps 0-7
 constexpr int kSoftmaxThreads = kSoftmaxWarps * 32;
-constexpr int kOwnWarp0 = 8;              // warps 8, 9: Q + records
-constexpr int kOwnWarps = 2;
+constexpr int kOwnWarp0 = 8;              // warp 8: Q + records
+constexpr int kOwnWarps = 1;
+constexpr int kPvMmaWarp = 9;             // CTA 0: issues PV
 constexpr int kPvWarp0 = 10;              // warp 10: peer keys' value dims
 constexpr int kPvWarps = 1;
-constexpr int kMmaWarp = 11;
+constexpr int kMmaWarp = 11;              // allocates TMEM; CTA 0: issues QK
 constexpr int kThreads = 12 * 32;
 constexpr uint32_t kQBytes = kChunks * kQChunkBytes;
 constexpr uint32_t kOwnBytes = kChunks * kKeyChunkBytes;  // records of a CTA's 32 keys
@@ -164,17 +165,6 @@ __device__ __forceinline__ uint64_t umma_desc_sw64(uint32_t addr) {
 // Arrive on the mbarrier at shared::cluster address `bar` once the pair's previously issued MMAs complete.
 __device__ __forceinline__ void commit_pair(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ bool mbar_test_cluster(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
 }
 // Every thread of the barrier gets the OR of the predicates.
 template <int ID>
@@ -418,13 +408,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == kMmaWarp) {
     if (crank == 0 && elect_one()) {
-      // ------------------------------------------------------- MMA issuer
+      // ------------------------------------------------------ QK issuer
+      // QK and PV are issued by threads of their own, so that neither waits
+      // for the other's operands or polls for them.
       const uint32_t idesc_qk = umma_idesc(128, BN, 1, 1);
-      const uint32_t idesc_pv = umma_idesc(128, 256, 1, 1) | (1u << 16);  // B (V) MN-major
-      auto peer = [&](uint64_t* bar) { return mapa_shared(smem_u32(bar), 1); };
       bool ok = mbar_wait_cluster(&s.q_full, 0, err, kErrTimeoutTmaFull, abort_flag);
-      auto issue_qk = [&](int i) {
+      for (int i = 0; i < ntiles && ok; ++i) {
         const int st = i % STAGES, b = i % SBUF;
+        ok = mbar_wait_cluster(&s.s_empty[b], ((i / SBUF) & 1) ^ 1, err, kErrTimeoutTmemEmpty, abort_flag) &&
+             mbar_wait_cluster(&s.own_full[st], (i / STAGES) & 1, err, kErrTimeoutTmaFull, abort_flag);
+        if (!ok) break;
         fence_proxy_async();  // cp.async rows (generic proxy) before the tensor core reads them
         tc_fence_after();
         const uint32_t d = tmem + kTmemS + b * (BN / 2);
@@ -437,10 +430,19 @@ __global__ void __launch_bounds__(kThreads, 1)
             mma_pair_ss(d, adesc + ((k * 32) >> 4), bdesc + ((k * 32) >> 4), idesc_qk, (j > 0 || k > 0) ? 1u : 0u);
         }
         commit_pair(smem_u32(&s.s_full[b]));
-        commit_pair(peer(&s.s_full[b]));
-      };
-      auto issue_pv = [&](int i) {
+        commit_pair(mapa_shared(smem_u32(&s.s_full[b]), 1));
+      }
+    }
+  } else if (warp == kPvMmaWarp) {
+    if (crank == 0 && elect_one()) {
+      // ------------------------------------------------------ PV issuer
+      const uint32_t idesc_pv = umma_idesc(128, 256, 1, 1) | (1u << 16);  // B (V) MN-major
+      bool ok = true;
+      for (int i = 0; i < ntiles && ok; ++i) {
         const int st = i % STAGES;
+        ok = mbar_wait_cluster(&s.pv_full[st], (i / STAGES) & 1, err, kErrTimeoutTmaFull, abort_flag) &&
+             mbar_wait_cluster(&s.p_full[i % PBUF], (i / PBUF) & 1, err, kErrTimeoutGeneric, abort_flag);
+        if (!ok) break;
         fence_proxy_async();
         tc_fence_after();
 #pragma unroll
@@ -454,35 +456,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         commit_pair(smem_u32(&s.pv_done[st]));
-        commit_pair(peer(&s.pv_done[st]));
-      };
-      int nq = 0, np = 0;
-      uint64_t idle_since = 0;
-      while (ok && np < ntiles) {
-        bool progressed = false;
-        if (nq < ntiles && mbar_test_cluster(&s.own_full[nq % STAGES], (nq / STAGES) & 1) &&
-            mbar_test_cluster(&s.s_empty[nq % SBUF], ((nq / SBUF) & 1) ^ 1)) {
-          issue_qk(nq++);
-          progressed = true;
-        }
-        if (np < nq && mbar_test_cluster(&s.p_full[np % PBUF], (np / PBUF) & 1) &&
-            mbar_test_cluster(&s.pv_full[np % STAGES], (np / STAGES) & 1)) {
-          issue_pv(np++);
-          progressed = true;
-        }
-        if (progressed) {
-          idle_since = 0;
-        } else if (idle_since == 0) {
-          idle_since = globaltimer_ns();
-        } else if (globaltimer_ns() - idle_since > kWaitBudgetNs || *abort_flag) {
-          record_error(err, kErrTimeoutGeneric);
-          *abort_flag = 1;
-          ok = false;
-        }
+        commit_pair(mapa_shared(smem_u32(&s.pv_done[st]), 1));
       }
       if (ok) {
         commit_pair(smem_u32(&s.o_full));
-        commit_pair(peer(&s.o_full));
+        commit_pair(mapa_shared(smem_u32(&s.o_full), 1));
       }
     }
   }
@@ -505,9 +483,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int b = i % SBUF;
       const int rb = (i >> 1) & 1;
       const int valid = tile_valid(i) - BNC * kh;  // this thread's keys j < valid count
-      bool got = __all_sync(0xffffffffu, mbar_wait(&s.s_full[b], (i / SBUF) & 1, err, kErrTimeoutTmemFull, abort_flag));
+      // The running maximum after tile i - 1 comes from the other warpgroup, which has published it long
+      // before it is done with that tile.
+      bool clear = true;
+      float m_prev = -INFINITY;
+      if (i > 0) {
+        clear = __all_sync(0xffffffffu, mbar_wait(&s.m_ready[(i - 1) & 1], ((i - 1) >> 1) & 1, err, kErrTimeoutGeneric,
+                                                  abort_flag));
+        m_prev = s.m_run[(i - 1) & 1][hrow];
+      }
+      clear &= __all_sync(0xffffffffu, mbar_wait(&s.s_full[b], (i / SBUF) & 1, err, kErrTimeoutTmemFull, abort_flag));
       uint32_t r[32];
-      if (got) {
+      if (clear) {
         tc_fence_after();
         tmem_ld32(tmem + lane_addr + kTmemS + b * (BN / 2), r);
         tmem_wait_ld();
@@ -532,24 +519,35 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int j = 0; j < 4; ++j) mx[j] = fmaxf(mx[j], mx[j + 4]);
       float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2;  // the scale is positive
-      s.red[rb][tt] = mt;
-      const bool fail = wg == 0 ? bar_red_or<1>(kSoftmaxThreads / 2, !got || pending_fail)
-                                : bar_red_or<2>(kSoftmaxThreads / 2, !got || pending_fail);
-      if (fail) {
-        failed = true;
-        break;
+      uint32_t pk[16];
+      float sum;
+      auto weights = [&](float m) {
+        const float mbase = m == -INFINITY ? 0.f : m;
+        float ps[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float x = ex2_approx(fmaf(__uint_as_float(r[2 * j]), scale_log2, -mbase));
+          const float y = ex2_approx(fmaf(__uint_as_float(r[2 * j + 1]), scale_log2, -mbase));
+          ps[j & 3] += x + y;
+          pk[j] = pack_bf16(x, y);
+        }
+        sum = (ps[0] + ps[1]) + (ps[2] + ps[3]);
+      };
+      // Usually no row's maximum grows by the threshold and the weights relative to the old one stand.
+      weights(m_prev);
+      float m = m_prev;
+      const bool grows = m_prev == -INFINITY ? mt > -INFINITY : mt > m_prev + kRescaleThreshold;
+      const bool stop = !clear || pending_fail;
+      if (wg == 0 ? bar_red_or<1>(kSoftmaxThreads / 2, grows || stop) : bar_red_or<2>(kSoftmaxThreads / 2, grows || stop)) {
+        s.red[rb][tt] = mt;
+        if (wg == 0 ? bar_red_or<1>(kSoftmaxThreads / 2, stop) : bar_red_or<2>(kSoftmaxThreads / 2, stop)) {
+          failed = true;
+          break;
+        }
+        mt = fmaxf(mt, s.red[rb][tt ^ 64]);
+        if (m_prev == -INFINITY || mt > m_prev + kRescaleThreshold) m = mt;
+        weights(m);
       }
-      mt = fmaxf(mt, s.red[rb][tt ^ 64]);
-      // The running maximum after tile i - 1 comes from the other warpgroup, which has published it long
-      // before it is done with that tile.
-      float m_prev = -INFINITY;
-      bool clear = true;
-      if (i > 0) {
-        clear = __all_sync(0xffffffffu, mbar_wait(&s.m_ready[(i - 1) & 1], ((i - 1) >> 1) & 1, err, kErrTimeoutGeneric,
-                                                  abort_flag));
-        m_prev = s.m_run[(i - 1) & 1][hrow];
-      }
-      const float m = (m_prev == -INFINITY || mt > m_prev + kRescaleThreshold) ? mt : m_prev;
       if (kh == 0) s.m_run[i & 1][hrow] = m;  // both threads of the row hold the same value
       // (lanes r and r + 64 are different warps: each warp's arrival follows its own writes)
       __syncwarp();
@@ -560,19 +558,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         l = m_used == -INFINITY ? 0.f : l * exp2f(m_used - m);
         m_used = m;
       }
-      const float mbase = m == -INFINITY ? 0.f : m;
-      uint32_t pk[16];
-      float ps[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float x = ex2_approx(fmaf(__uint_as_float(r[2 * j]), scale_log2, -mbase));
-        const float y = ex2_approx(fmaf(__uint_as_float(r[2 * j + 1]), scale_log2, -mbase));
-        ps[j & 3] += x + y;
-        pk[j] = pack_bf16(x, y);
-      }
-      l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+      l += sum;
       // P(i) reuses the buffer of P(i - PBUF): wait for its PV.
-      if (clear && i >= PBUF)
+      if (i >= PBUF)
         clear = __all_sync(0xffffffffu, mbar_wait(&s.pv_done[(i - PBUF) % STAGES], ((i - PBUF) / STAGES) & 1, err,
                                                   kErrTimeoutTmemEmpty, abort_flag));
       if (clear && __any_sync(0xffffffffu, rescale)) {
