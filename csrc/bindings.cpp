@@ -403,91 +403,108 @@ void sparse_mla(const Tensor& q, const Tensor& kv, const Tensor& ids, double sca
 }
 
 // --------------------------------------------- continuations of one history
-// q [B,T,H,576] over prefix [P,576] plus the visible rows of tail [B,S,576].
-void shared_prefix_mla(const Tensor& q, const Tensor& prefix, const c10::optional<Tensor>& tail,
-                       const c10::optional<Tensor>& tail_lens, double scale, Tensor& out,
-                       const c10::optional<Tensor>& lse) {
-  CHECK_CUDA(q); CHECK_CUDA(prefix); CHECK_CUDA(out);
-  CHECK_DTYPE(q, torch::kBFloat16); CHECK_DTYPE(prefix, torch::kBFloat16); CHECK_DTYPE(out, torch::kBFloat16);
-  TORCH_CHECK(q.dim() == 4 && q.size(3) == 576 && q.is_contiguous(), "shared_prefix_mla: q [B,T,H,576]");
-  TORCH_CHECK(out.dim() == 4 && out.is_contiguous() && out.size(0) == q.size(0) && out.size(1) == q.size(1) &&
-                  out.size(2) == q.size(2) && out.size(3) == 512, "shared_prefix_mla: out [B,T,H,512]");
-  auto rows_ok = [](const Tensor& t) {  // records of 576 dims on 16-byte boundaries
-    bool ok = t.size(-1) == 576 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
-    if (t.numel() == 0) return ok;
-    ok = ok && t.stride(-1) == 1;
-    for (int64_t d = 0; d + 1 < t.dim(); ++d) ok = ok && (t.size(d) == 1 || (t.stride(d) >= 0 && t.stride(d) % 8 == 0));
-    return ok;
-  };
-  TORCH_CHECK(prefix.dim() == 2 && rows_ok(prefix) && prefix.size(0) < (int64_t(1) << 31),
-              "shared_prefix_mla: prefix [P,576], rows 16-byte aligned");
-  TORCH_CHECK(prefix.device() == q.device() && out.device() == q.device(), "shared_prefix_mla: one device");
-  c10::cuda::CUDAGuard g(q.device());
-  b200::PrefixMLAArgs a{};
-  a.q = cptr<__nv_bfloat16>(q); a.prefix = cptr<__nv_bfloat16>(prefix); a.out = ptr<__nv_bfloat16>(out);
-  a.B = q.size(0); a.T = q.size(1); a.H = q.size(2); a.P = prefix.size(0); a.scale = float(scale);
-  a.ld_prefix = prefix.size(0) > 1 ? prefix.stride(0) : 576;
-  a.err = err_ptr(q);
-  if (tail && tail->defined()) {
-    CHECK_DTYPE((*tail), torch::kBFloat16);
-    TORCH_CHECK(tail->dim() == 3 && tail->size(0) == q.size(0) && rows_ok(*tail) && tail->device() == q.device(),
-                "shared_prefix_mla: tail [B,S,576], rows 16-byte aligned");
-    a.tail = cptr<__nv_bfloat16>(*tail);
-    a.S = tail->size(1); a.ld_batch = tail->stride(0); a.ld_tail = tail->stride(1);
-    if (tail_lens && tail_lens->defined()) {
-      CHECK_DTYPE((*tail_lens), torch::kInt32);
-      TORCH_CHECK(tail_lens->is_contiguous() && tail_lens->dim() == 1 && tail_lens->size(0) == q.size(0) &&
-                      tail_lens->device() == q.device(), "shared_prefix_mla: tail_lens [B] int32");
-      a.tail_lens = cptr<int>(*tail_lens);
-    }
-  }
-  if (lse && lse->defined()) {
-    CHECK_DTYPE((*lse), torch::kFloat32);
-    TORCH_CHECK(lse->is_contiguous() && lse->numel() == q.size(0) * q.size(1) * q.size(2), "shared_prefix_mla: lse");
-    a.lse = ptr<float>(*lse);
-  }
-  Tensor scratch;
-  const size_t floats = b200::shared_prefix_mla_scratch_floats(a);
-  if (floats) scratch = torch::empty({int64_t(floats)}, torch::dtype(torch::kFloat32).device(q.device()));
-  b200::launch_shared_prefix_mla(a, floats ? scratch.data_ptr<float>() : nullptr, stream());
+// Arguments that a caller can get wrong raise ValueError (std::invalid_argument).
+#define CHECK_VALUE(cond, msg) \
+  do { if (!(cond)) throw std::invalid_argument(msg); } while (0)
+
+// Rows the kernels can load: contiguous records that start on 16-byte boundaries.
+bool records_ok(const Tensor& t) {
+  if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) return false;
+  if (t.numel() == 0) return true;
+  if (t.stride(-1) != 1) return false;
+  for (int64_t d = 0; d + 1 < t.dim(); ++d)
+    if (t.size(d) > 1 && (t.stride(d) < 0 || t.stride(d) % 8)) return false;
+  return true;
 }
 
-void sample_tokens(const Tensor& logits, const Tensor& u, const c10::optional<Tensor>& temperature,
-                   const c10::optional<Tensor>& top_k, const c10::optional<Tensor>& top_p,
-                   const c10::optional<Tensor>& min_p, double temperature0, int64_t top_k0, double top_p0,
-                   double min_p0, Tensor& tokens, Tensor& logprobs) {
-  CHECK_CUDA(logits); CHECK_DTYPE(u, torch::kFloat32); CHECK_DTYPE(tokens, torch::kInt64);
-  CHECK_DTYPE(logprobs, torch::kFloat32);
-  TORCH_CHECK(logits.scalar_type() == torch::kFloat32 || logits.scalar_type() == torch::kBFloat16,
-              "sample_tokens: logits FP32 or BF16");
-  TORCH_CHECK(logits.dim() == 2 && logits.size(1) >= 1 && (logits.size(1) == 1 || logits.stride(1) == 1) &&
-                  logits.stride(0) >= 0, "sample_tokens: logits [R,V], contiguous in the vocabulary");
-  TORCH_CHECK(logits.size(1) <= b200::sample_max_vocabulary(), "sample_tokens: vocabulary too large");
+// q [B,H,576] or [B,T,H,576] over prefix [P,576] plus the visible rows of tail [B,S,576].
+std::tuple<Tensor, c10::optional<Tensor>> shared_prefix_mla(const Tensor& q, const Tensor& prefix,
+                                                            const c10::optional<Tensor>& tail,
+                                                            const c10::optional<Tensor>& tail_lens, double scale,
+                                                            bool want_lse) {
+  CHECK_CUDA(q);
+  const int64_t B = q.size(0), T = q.dim() == 4 ? q.size(1) : 1, H = q.size(-2);
+  CHECK_VALUE(q.scalar_type() == torch::kBFloat16 && prefix.scalar_type() == torch::kBFloat16 &&
+                  (!tail || tail->scalar_type() == torch::kBFloat16),
+              "q, prefix and tail must be BF16");
+  CHECK_VALUE(q.size(-1) == 576 && prefix.size(-1) == 576 && (!tail || tail->size(-1) == 576),
+              "the sm_100a shared-prefix MLA kernel covers the V3.2 shape (576 / 512)");
+  CHECK_VALUE(prefix.device() == q.device() && (!tail || tail->device() == q.device()) &&
+                  (!tail_lens || tail_lens->device() == q.device()),
+              "q, prefix, tail and tail_lens must be on one device");
+  CHECK_VALUE(records_ok(prefix), "prefix records must be contiguous and start on 16-byte boundaries");
+  CHECK_VALUE(!tail || records_ok(*tail), "tail records must be contiguous and start on 16-byte boundaries");
+  CHECK_VALUE(!tail_lens || tail_lens->scalar_type() == torch::kInt32, "tail_lens must be int32");
+  CHECK_VALUE(B * T * H < (int64_t(1) << 31) - 256 && prefix.size(0) < (int64_t(1) << 31) - 256 &&
+                  (!tail || tail->size(1) < (int64_t(1) << 30)),
+              "more rows than 32-bit indices hold");
+  c10::cuda::CUDAGuard g(q.device());
+  const Tensor qc = q.contiguous();
+  if (reinterpret_cast<uintptr_t>(qc.data_ptr()) % 16) throw std::invalid_argument("q must start on a 16-byte boundary");
+  auto shape = q.sizes().vec();
+  shape.back() = 512;
+  Tensor out = torch::empty(shape, q.options());
+  c10::optional<Tensor> lse;
+  shape.pop_back();
+  if (want_lse) lse = torch::empty(shape, q.options().dtype(torch::kFloat32));
+  const Tensor lens = tail_lens ? tail_lens->contiguous() : Tensor();
+  b200::PrefixMLAArgs a{};
+  a.q = cptr<__nv_bfloat16>(qc); a.prefix = cptr<__nv_bfloat16>(prefix); a.out = ptr<__nv_bfloat16>(out);
+  a.B = B; a.T = T; a.H = H; a.P = prefix.size(0); a.scale = float(scale);
+  a.ld_prefix = prefix.size(0) > 1 ? prefix.stride(0) : 576;
+  a.err = err_ptr(q);
+  if (tail) {
+    a.tail = cptr<__nv_bfloat16>(*tail);
+    a.S = tail->size(1); a.ld_batch = tail->stride(0); a.ld_tail = tail->stride(1);
+    if (tail_lens) a.tail_lens = cptr<int>(lens);
+  }
+  if (lse) a.lse = ptr<float>(*lse);
+  Tensor scratch;
+  b200::launch_shared_prefix_mla(
+      a,
+      [&](size_t n) {
+        scratch = torch::empty({int64_t(n)}, q.options().dtype(torch::kFloat32));
+        return scratch.data_ptr<float>();
+      },
+      stream());
+  return {out, lse};
+}
+
+std::tuple<Tensor, Tensor> sample_tokens(const Tensor& logits_, const Tensor& u, const c10::optional<Tensor>& temperature,
+                                         const c10::optional<Tensor>& top_k, const c10::optional<Tensor>& top_p,
+                                         const c10::optional<Tensor>& min_p, double temperature0, int64_t top_k0,
+                                         double top_p0, double min_p0) {
+  CHECK_CUDA(logits_);
+  CHECK_VALUE(logits_.size(1) <= b200::sample_max_vocabulary(),
+              "the sampling kernel takes vocabularies of up to " + std::to_string(b200::sample_max_vocabulary()));
+  c10::cuda::CUDAGuard g(logits_.device());
+  const Tensor logits = logits_.size(1) == 1 || logits_.stride(1) == 1 ? logits_ : logits_.contiguous();
   const int64_t R = logits.size(0);
-  auto per_row = [&](const Tensor& t, const char* what) {
-    TORCH_CHECK(t.dim() == 1 && t.size(0) == R && t.is_contiguous() && t.device() == logits.device(),
-                "sample_tokens: ", what, " must be a contiguous [R] tensor on the logits' device");
+  CHECK_VALUE(R < (int64_t(1) << 27), "sample_tokens: too many rows");
+  auto per_row = [&](const c10::optional<Tensor>& t, c10::ScalarType type, const char* what) -> Tensor {
+    if (!t) return Tensor();
+    if (t->dim() != 1 || t->size(0) != R || t->device() != logits.device() || t->scalar_type() != type)
+      throw std::invalid_argument(std::string(what) + " must be a number or an [R] " + c10::toString(type) +
+                                  " tensor on the logits' device");
+    return t->contiguous();
   };
-  per_row(u, "u"); per_row(tokens, "tokens"); per_row(logprobs, "logprobs");
-  c10::cuda::CUDAGuard g(logits.device());
+  const Tensor ut = per_row(u, torch::kFloat32, "u"), t = per_row(temperature, torch::kFloat32, "temperature"),
+               kt = per_row(top_k, torch::kInt32, "top_k"), pt = per_row(top_p, torch::kFloat32, "top_p"),
+               mt = per_row(min_p, torch::kFloat32, "min_p");
+  Tensor tokens = torch::empty({R}, u.options().dtype(torch::kInt64));
+  Tensor logprobs = torch::empty({R}, u.options());
   b200::SampleArgs a{};
   a.logits = logits.data_ptr(); a.bf16 = logits.scalar_type() == torch::kBFloat16; a.ld = logits.stride(0);
-  a.R = R; a.V = logits.size(1); a.u = cptr<float>(u);
-  auto floats = [&](const c10::optional<Tensor>& t, const char* what) -> const float* {
-    if (!t || !t->defined()) return nullptr;
-    CHECK_DTYPE((*t), torch::kFloat32);
-    per_row(*t, what);
-    return cptr<float>(*t);
-  };
-  a.temperature = floats(temperature, "temperature"); a.top_p = floats(top_p, "top_p"); a.min_p = floats(min_p, "min_p");
-  if (top_k && top_k->defined()) {
-    CHECK_DTYPE((*top_k), torch::kInt32);
-    per_row(*top_k, "top_k");
-    a.top_k = cptr<int>(*top_k);
-  }
-  a.temperature0 = float(temperature0); a.top_p0 = float(top_p0); a.min_p0 = float(min_p0); a.top_k0 = int(top_k0);
+  a.R = R; a.V = logits.size(1); a.u = cptr<float>(ut);
+  if (t.defined()) a.temperature = cptr<float>(t);
+  if (kt.defined()) a.top_k = cptr<int>(kt);
+  if (pt.defined()) a.top_p = cptr<float>(pt);
+  if (mt.defined()) a.min_p = cptr<float>(mt);
+  a.temperature0 = float(temperature0); a.top_p0 = float(top_p0); a.min_p0 = float(min_p0);
+  a.top_k0 = int(std::min<int64_t>(top_k0, INT32_MAX));
   a.tokens = ptr<int64_t>(tokens); a.logprobs = ptr<float>(logprobs);
   b200::launch_sample_tokens(a, stream());
+  return {tokens, logprobs};
 }
 
 Tensor topk_trace(int64_t row) {

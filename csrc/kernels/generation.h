@@ -4,10 +4,25 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstddef>
 #include <cstdint>
+#include <functional>
 
 namespace b200 {
+
+// Run f the first time the current device reaches this point (Tag names the point); f may run twice when
+// two threads reach it together, so it must be repeatable.
+template <typename Tag, typename F>
+void once_per_device(F&& f) {
+  static std::atomic<uint64_t> done{0};
+  int device = 0;
+  cudaGetDevice(&device);
+  const uint64_t bit = 1ull << (device & 63);
+  if (done.load(std::memory_order_acquire) & bit) return;
+  f();
+  done.fetch_or(bit, std::memory_order_release);
+}
 
 // ------------------------------------------------------- shared-prefix MLA
 struct PrefixMLAArgs {
@@ -22,9 +37,9 @@ struct PrefixMLAArgs {
   float scale;
   int* err;
 };
-// FP32 workspace of a call (0: none); the same arguments give the same plan.
-size_t shared_prefix_mla_scratch_floats(const PrefixMLAArgs& a);
-void launch_shared_prefix_mla(const PrefixMLAArgs& a, float* scratch, cudaStream_t stream);
+// `workspace(n)` returns n floats that live until the call's kernels are done (asked for at most once).
+void launch_shared_prefix_mla(const PrefixMLAArgs& a, const std::function<float*(size_t)>& workspace,
+                              cudaStream_t stream);
 
 // ---------------------------------------------------------------- sampling
 struct SampleArgs {

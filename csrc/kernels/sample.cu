@@ -900,8 +900,13 @@ void launch_sample_tokens(const SampleArgs& a, cudaStream_t stream) {
   const int chunk = (slice_positions(a.V, C) + kWarps * kStep - 1) / (kWarps * kStep) * kStep;
   const size_t smem = sizeof(Shared) + size_t(chunk) * kWarps * 4;
   auto kernel = a.bf16 ? sample_kernel<true> : sample_kernel<false>;
-  cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)), "sample_tokens smem");
-  cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "sample_tokens cluster");
+  once_per_device<Shared>([] {
+    for (auto* k : {sample_kernel<true>, sample_kernel<false>}) {
+      cuda_check(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(Shared) + kSlice * 4)),
+                 "sample_tokens smem");
+      cuda_check(cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "sample_tokens cluster");
+    }
+  });
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(a.R) * C, 1, 1);
   cfg.blockDim = dim3(kThreads, 1, 1);

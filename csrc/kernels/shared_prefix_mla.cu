@@ -261,7 +261,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                       float scale_log2, float* __restrict__ part_o,
                       float* __restrict__ part_lse) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  pdl_wait();
   uint8_t* base = smem_raw;
   const uint32_t sbase = smem_u32(base);
   if (sbase & 1023u) {  // uniform over the cluster; the swizzle atoms need it and there is no room for slack
@@ -270,22 +269,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   Small& s = *reinterpret_cast<Small*>(base + kOffSmall);
   const uint32_t crank = cluster_ctarank();
-  const Unit w = decode_unit(a, plan, int(blockIdx.x >> 1));
-  const int ntiles = w.ntiles();
   const int warp = threadIdx.x / 32;
   const int lane = threadIdx.x % 32;
-
-  auto own_chunk = [&](int st, int j) { return sbase + kOffOwn + (st * kChunks + j) * kKeyChunkBytes; };
-  // PV's B operand (value dims, MN-major) of key half kh and value half v.
-  auto pv_region = [&](int st, int kh, int v) { return own_chunk(st, 4 * v + 2 * kh); };
-  // P of tile i in two K halves (64-byte swizzle): keys [0, 32) take the tile's record chunk of the RoPE dims,
-  // which only QK needed, keys [32, 64) a buffer of their own.
-  auto p_half = [&](int i, int kh) {
-    return kh == 0 ? own_chunk(i % STAGES, kChunks - 1) : sbase + kOffP + (i % PBUF) * kPBytes;
-  };
-  // Tile i: first key row of its source (prefix or tail) and how many of its 64 keys are visible.
-  auto tile_key0 = [&](int i) { return (i < w.np ? w.p0 + i : w.t0 + i - w.np) * BN; };
-  auto tile_valid = [&](int i) { return min(BN, (i < w.np ? a.P : w.seen) - tile_key0(i)); };
 
   if (threadIdx.x == 0) {
     mbar_init(&s.q_full, 2);
@@ -311,8 +296,23 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();  // both CTAs' barriers initialised before any remote arrive
+  // What came before this line overlaps the previous kernel; TMEM is held, so the next one may start.
+  pdl_wait();
   pdl_trigger();
   tc_fence_after();
+  const Unit w = decode_unit(a, plan, int(blockIdx.x >> 1));
+  const int ntiles = w.ntiles();
+  auto own_chunk = [&](int st, int j) { return sbase + kOffOwn + (st * kChunks + j) * kKeyChunkBytes; };
+  // PV's B operand (value dims, MN-major) of key half kh and value half v.
+  auto pv_region = [&](int st, int kh, int v) { return own_chunk(st, 4 * v + 2 * kh); };
+  // P of tile i in two K halves (64-byte swizzle): keys [0, 32) take the tile's record chunk of the RoPE dims,
+  // which only QK needed, keys [32, 64) a buffer of their own.
+  auto p_half = [&](int i, int kh) {
+    return kh == 0 ? own_chunk(i % STAGES, kChunks - 1) : sbase + kOffP + (i % PBUF) * kPBytes;
+  };
+  // Tile i: first key row of its source (prefix or tail) and how many of its 64 keys are visible.
+  auto tile_key0 = [&](int i) { return (i < w.np ? w.p0 + i : w.t0 + i - w.np) * BN; };
+  auto tile_valid = [&](int i) { return min(BN, (i < w.np ? a.P : w.seen) - tile_key0(i)); };
   const uint32_t tmem = s.tmem_base;
   volatile int* abort_flag = &s.abort_flag;
   int* err = a.err;
@@ -323,6 +323,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
   const uint8_t* tail_rows = reinterpret_cast<const uint8_t*>(a.tail + int64_t(w.b) * a.ld_batch);
   const int64_t tail_pitch = a.ld_tail * 2;
+  // Rows [rows, 32) of key half kh's value dims in this CTA (one warp; 32 units of 16 bytes per row).
+  auto zero_value_rows = [&](int st, int kh, int rows) {
+    for (int r = rows; r < BNC; ++r) {
+      const uint32_t dst = pv_region(st, kh, lane >> 4) + ((lane >> 3) & 1) * kKeyChunkBytes + r * 128 + (lane & 7) * 16;
+      asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(0) : "memory");
+    }
+  };
 
   if (ntiles == 0) {
     // nothing visible: straight to the epilogue
@@ -353,13 +360,20 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       } else {
-#pragma unroll 4
-        for (int e = ow * 32 + lane; e < BNC * 72; e += kOwnWarps * 32) {
-          const int r = e / 72, u72 = e % 72;
-          const bool ok = key0 + r < w.seen;
-          const uint32_t dst = own_chunk(st, u72 >> 3) + r * 128 + (((u72 & 7) ^ (r & 7)) << 4);
-          cp_async16_zfill(dst, ok ? tail_rows + int64_t(key0 + r) * tail_pitch + u72 * 16 : tail_rows, ok);
+        // Visible rows by cp.async; of the others only the value dims have to be finite (their scores are
+        // masked, but 0 * NaN would spread in PV): zeros.
+        const int rows = min(max(w.seen - key0, 0), BNC);
+#pragma unroll 2
+        for (int r = 0; r < rows; ++r) {
+          const uint8_t* src = tail_rows + int64_t(key0 + r) * tail_pitch;
+#pragma unroll
+          for (int e = 0; e < 3; ++e) {
+            const int u72 = lane + 32 * e;
+            if (u72 < 72)
+              cp_async16_zfill(own_chunk(st, u72 >> 3) + r * 128 + (((u72 & 7) ^ (r & 7)) << 4), src + u72 * 16, true);
+          }
         }
+        zero_value_rows(st, int(crank), rows);
         cp_async_wait_all();
         fence_proxy_async();
         __syncwarp();
@@ -391,14 +405,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       } else {
-#pragma unroll 4
-        for (int e = pw * 32 + lane; e < BNC * 32; e += kPvWarps * 32) {
-          const int r = e >> 5, v = (e >> 4) & 1, qc = (e >> 3) & 1, u = e & 7;
-          const bool ok = key0 + r < w.seen;
-          const uint32_t dst = pv_region(st, peer, v) + qc * kKeyChunkBytes + r * 128 + ((u ^ (r & 7)) << 4);
-          const int unit = (4 * v + 2 * int(crank) + qc) * 8 + u;
-          cp_async16_zfill(dst, ok ? tail_rows + int64_t(key0 + r) * tail_pitch + unit * 16 : tail_rows, ok);
-        }
+        const int rows = min(max(w.seen - key0, 0), BNC);
+        const int v = lane >> 4, qc = (lane >> 3) & 1, u = lane & 7;
+        const int unit = (4 * v + 2 * int(crank) + qc) * 8 + u;
+#pragma unroll 2
+        for (int r = 0; r < rows; ++r)
+          cp_async16_zfill(pv_region(st, peer, v) + qc * kKeyChunkBytes + r * 128 + ((u ^ (r & 7)) << 4),
+                           tail_rows + int64_t(key0 + r) * tail_pitch + unit * 16, true);
+        zero_value_rows(st, peer, rows);
         cp_async_wait_all();
         fence_proxy_async();
         __syncwarp();
@@ -520,7 +534,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int j = 0; j < 4; ++j) mx[j] = fmaxf(mx[j], mx[j + 4]);
       float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2;  // the scale is positive
       uint32_t pk[16];
-      float sum;
+      float sum = 0.f;
       auto weights = [&](float m) {
         const float mbase = m == -INFINITY ? 0.f : m;
         float ps[4] = {0.f, 0.f, 0.f, 0.f};
@@ -534,9 +548,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         sum = (ps[0] + ps[1]) + (ps[2] + ps[3]);
       };
       // Usually no row's maximum grows by the threshold and the weights relative to the old one stand.
-      weights(m_prev);
+      if (i > 0) weights(m_prev);
       float m = m_prev;
-      const bool grows = m_prev == -INFINITY ? mt > -INFINITY : mt > m_prev + kRescaleThreshold;
+      const bool grows = i == 0 || (m_prev == -INFINITY ? mt > -INFINITY : mt > m_prev + kRescaleThreshold);
       const bool stop = !clear || pending_fail;
       if (wg == 0 ? bar_red_or<1>(kSoftmaxThreads / 2, grows || stop) : bar_red_or<2>(kSoftmaxThreads / 2, grows || stop)) {
         s.red[rb][tt] = mt;
@@ -617,14 +631,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     // A row without visible keys has sum 0; NaN scores stay NaN.
     const float inv = lt == 0.f ? 0.f : 1.f / lt;
     const float lse = lt == 0.f ? -INFINITY : (m_last == -INFINITY ? 0.f : m_last) * 0.69314718055994531f + logf(lt);
-    const bool have_o = !any_fail && ntiles > 0 &&
-                        __all_sync(0xffffffffu, mbar_wait(&s.o_full, 0, err, kErrTimeoutTmemFull, abort_flag));
+    const bool got_o = !any_fail && ntiles > 0 &&
+                       __all_sync(0xffffffffu, mbar_wait(&s.o_full, 0, err, kErrTimeoutTmemFull, abort_flag));
+    const bool have_o = !bar_red_or<3>(kSoftmaxThreads, !got_o);  // all or none: barriers follow
     if (have_o) tc_fence_after();
     const int trow = MC * int(crank) + hrow;  // row within the tile
     const int64_t row = w.row0 + trow;
-    const bool store = trow < w.nrows;
-    // Warpgroup wg owns value half wg: columns [128 wg, +128) = dims 256 wg + 128 kh + [0, 128).
+    // O leaves through shared memory (the operands are no longer needed), so that a warp writes whole rows:
+    // straight from the registers every store would touch 32 rows.  16-byte units are XORed with the row.
+    // Warpgroup wg holds value half wg: columns [128 wg, +128) = dims 256 wg + 128 kh + [0, 128).
     if (w.slot < 0 || have_o) {
+      const uint32_t stage = sbase + (w.slot < 0 ? kOffQ : kOffOwn);
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         uint32_t r[32];
@@ -637,28 +654,44 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int j = 0; j < 32; ++j) r[j] = 0u;
         }
         const int dim0 = 256 * wg + 128 * kh + 32 * c;
-        if (w.slot >= 0) {
-          // [slot][dim][row]: a warp's store is one 128-byte line.
-          float* o = part_o + (int64_t(w.slot) * DV + dim0) * BM + trow;
+        auto scaled = [&](int j) { return __uint_as_float(r[j]) * inv; };
+        if (w.slot < 0) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) o[j * BM] = __uint_as_float(r[j]) * inv;
-        } else if (store) {
-          __nv_bfloat16* o = a.out + row * DV + dim0;
+          for (int j = 0; j < 32; j += 8)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
+                             stage + hrow * (DV * 2) + ((((dim0 + j) >> 3) ^ (hrow & 7)) << 4)),
+                         "r"(pack_bf16(scaled(j), scaled(j + 1))), "r"(pack_bf16(scaled(j + 2), scaled(j + 3))),
+                         "r"(pack_bf16(scaled(j + 4), scaled(j + 5))), "r"(pack_bf16(scaled(j + 6), scaled(j + 7)))
+                         : "memory");
+        } else {
 #pragma unroll
-          for (int j = 0; j < 32; j += 8) {
-            uint4 v;
-            v.x = pack_bf16(__uint_as_float(r[j]) * inv, __uint_as_float(r[j + 1]) * inv);
-            v.y = pack_bf16(__uint_as_float(r[j + 2]) * inv, __uint_as_float(r[j + 3]) * inv);
-            v.z = pack_bf16(__uint_as_float(r[j + 4]) * inv, __uint_as_float(r[j + 5]) * inv);
-            v.w = pack_bf16(__uint_as_float(r[j + 6]) * inv, __uint_as_float(r[j + 7]) * inv);
-            *reinterpret_cast<uint4*>(o + j) = v;
-          }
+          for (int j = 0; j < 32; j += 4)
+            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(
+                             stage + hrow * (DV * 4) + ((((dim0 + j) >> 2) ^ (hrow & 7)) << 4)),
+                         "f"(scaled(j)), "f"(scaled(j + 1)), "f"(scaled(j + 2)), "f"(scaled(j + 3))
+                         : "memory");
+        }
+      }
+      named_barrier(3, kSoftmaxThreads);
+      // One row of 16-byte units per warp and step: 64 units (BF16) or 128 (FP32 partials).
+      const int units = w.slot < 0 ? DV * 2 / 16 : DV * 4 / 16;
+      for (int rr = warp; rr < MC; rr += kSoftmaxWarps) {
+        const int tr = MC * int(crank) + rr;
+        if (w.slot < 0 && tr >= w.nrows) break;
+        uint8_t* dst = w.slot < 0 ? reinterpret_cast<uint8_t*>(a.out + (int64_t(w.row0) + tr) * DV)
+                                  : reinterpret_cast<uint8_t*>(part_o + (int64_t(w.slot) * BM + tr) * DV);
+        for (int u = lane; u < units; u += 32) {
+          uint4 q;
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w)
+                       : "r"(stage + rr * units * 16 + ((u ^ (rr & 7)) << 4)));
+          *reinterpret_cast<uint4*>(dst + u * 16) = q;
         }
       }
     }
     if (wg == 0 && kh == 0) {
       if (w.slot >= 0) part_lse[int64_t(w.slot) * BM + trow] = have_o ? lse : -INFINITY;
-      else if (a.lse && store) a.lse[row] = lse;
+      else if (a.lse && trow < w.nrows) a.lse[row] = lse;
     }
   }
 
@@ -677,14 +710,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // out[row] = sum_s exp(lse_s - lse) o_s over the partials of the row's tile
-// (and of its query's tail).  Thread = row, blockIdx.y = 8 value dims.
-__global__ void __launch_bounds__(BM) prefix_mla_merge_kernel(const __grid_constant__ PrefixMLAArgs a,
-                                                              const __grid_constant__ MergePlan mp,
-                                                              const float* __restrict__ part_o,
-                                                              const float* __restrict__ part_lse) {
+// (and of its query's tail).  A CTA per row, a thread per 4 value dims.
+__global__ void __launch_bounds__(DV / 4) prefix_mla_merge_kernel(const __grid_constant__ PrefixMLAArgs a,
+                                                                  const __grid_constant__ MergePlan mp,
+                                                                  const float* __restrict__ part_o,
+                                                                  const float* __restrict__ part_lse) {
   pdl_trigger();
   pdl_wait();
-  const int i = blockIdx.x, d0 = blockIdx.y * 8, lane = threadIdx.x;
+  const int i = blockIdx.x / BM, lane = blockIdx.x % BM, d0 = threadIdx.x * 4;
   const int64_t row = int64_t(mp.tile0 + i) * BM + lane;
   if (row >= int64_t(a.B) * a.T * a.H) return;
   int s0 = i, s1 = i + 1;
@@ -693,45 +726,42 @@ __global__ void __launch_bounds__(BM) prefix_mla_merge_kernel(const __grid_const
     s1 = mp.begin[i - mp.single + 1];
     if (s0 == s1) return;
   }
-  int64_t tail_slot = -1;
-  int tail_lane = 0;
+  int64_t tail = -1;  // row of the partials
   if (mp.apart) {
     const int g = int(row / a.H), h = int(row % a.H);
-    tail_slot = mp.tail_slot0 + int64_t(g) * ((a.H + BM - 1) / BM) + h / BM;
-    tail_lane = h % BM;
+    tail = (mp.tail_slot0 + int64_t(g) * ((a.H + BM - 1) / BM) + h / BM) * BM + h % BM;
   }
   float mx = -INFINITY;
   for (int s = s0; s < s1; ++s) mx = fmaxf(mx, part_lse[int64_t(s) * BM + lane]);
-  if (tail_slot >= 0) mx = fmaxf(mx, part_lse[tail_slot * BM + tail_lane]);
+  if (tail >= 0) mx = fmaxf(mx, part_lse[tail]);
   const float base = mx == -INFINITY ? 0.f : mx;
-  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float wsum = 0.f;
-  auto add = [&](int64_t slot, int l) {
-    const float lse = part_lse[slot * BM + l];
-    if (lse == -INFINITY) return;  // nothing visible there: its partial was not written
-    const float wt = expf(lse - base);
+  auto add = [&](int64_t r) {
+    const float lse = part_lse[r];
+    // -inf: nothing visible there, the partial was not written.
+    const float wt = lse == -INFINITY ? 0.f : expf(lse - base);
+    const float4 p = lse == -INFINITY ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                      : *reinterpret_cast<const float4*>(part_o + r * DV + d0);
     wsum += wt;
-    const float* p = part_o + (slot * DV + d0) * BM + l;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = fmaf(wt, p[j * BM], acc[j]);
+    acc.x = fmaf(wt, p.x, acc.x);
+    acc.y = fmaf(wt, p.y, acc.y);
+    acc.z = fmaf(wt, p.z, acc.z);
+    acc.w = fmaf(wt, p.w, acc.w);
   };
 #pragma unroll 4
-  for (int s = s0; s < s1; ++s) add(s, lane);
-  if (tail_slot >= 0) add(tail_slot, tail_lane);
+  for (int s = s0; s < s1; ++s) add(int64_t(s) * BM + lane);
+  if (tail >= 0) add(tail);
   const float inv = wsum == 0.f ? 0.f : 1.f / wsum;
-  uint4 v;
-  v.x = pack_bf16(acc[0] * inv, acc[1] * inv);
-  v.y = pack_bf16(acc[2] * inv, acc[3] * inv);
-  v.z = pack_bf16(acc[4] * inv, acc[5] * inv);
-  v.w = pack_bf16(acc[6] * inv, acc[7] * inv);
-  *reinterpret_cast<uint4*>(a.out + row * DV + d0) = v;
-  if (a.lse && blockIdx.y == 0) a.lse[row] = wsum == 0.f ? -INFINITY : base + logf(wsum);
+  *reinterpret_cast<uint2*>(a.out + row * DV + d0) =
+      make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+  if (a.lse && threadIdx.x == 0) a.lse[row] = wsum == 0.f ? -INFINITY : base + logf(wsum);
 }
 
 // How the row tiles are cut into shares.  Times in microseconds, measured on
 // B200: a 64-key tile, a share's start and end (launch, Q, filling the
 // pipeline, writing a partial), the merge kernel.
-constexpr double kTileUs = 0.65, kShareUs = 4., kMergeUs = 4.;
+constexpr double kTileUs = 0.8, kShareUs = 8., kMergeUs = 6.;
 constexpr int kMinShareTiles = 4;
 
 struct FullPlan {
@@ -802,22 +832,19 @@ void make_plan(const PrefixMLAArgs& a, FullPlan& f) {
 
 }  // namespace
 
-size_t shared_prefix_mla_scratch_floats(const PrefixMLAArgs& a) {
-  if (int64_t(a.B) * a.T * a.H == 0) return 0;
-  FullPlan f;
-  make_plan(a, f);
-  return size_t(f.plan.slots) * BM * (DV + 1);
-}
-
-void launch_shared_prefix_mla(const PrefixMLAArgs& a, float* scratch, cudaStream_t stream) {
+void launch_shared_prefix_mla(const PrefixMLAArgs& a, const std::function<float*(size_t)>& workspace,
+                              cudaStream_t stream) {
   const int64_t rows = int64_t(a.B) * a.T * a.H;
   if (rows == 0) return;
   FullPlan f;
   make_plan(a, f);
+  float* scratch = f.plan.slots ? workspace(size_t(f.plan.slots) * BM * (DV + 1)) : nullptr;
   const Plan& p = f.plan;
   static_assert(sizeof(Share) * kMaxShares + 512 < 32764, "kernel parameters");
-  cuda_check(cudaFuncSetAttribute(prefix_mla_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes)),
-             "shared_prefix_mla smem attribute");
+  once_per_device<FullPlan>([] {
+    cuda_check(cudaFuncSetAttribute(prefix_mla_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes)),
+               "shared_prefix_mla smem attribute");
+  });
   // Rows past the last one read zeros.  Without a prefix the map covers the queries (never loaded from).
   const CUtensorMap tq = make_tma_2d(a.q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, uint64_t(rows), D, uint64_t(D) * 2, 64, MC);
   const CUtensorMap tkv =
@@ -841,7 +868,7 @@ void launch_shared_prefix_mla(const PrefixMLAArgs& a, float* scratch, cudaStream
   cuda_check(cudaLaunchKernelEx(&cfg, prefix_mla_kernel, a, p, tq, tkv, a.scale * 1.4426950408889634f, scratch, part_lse),
              "shared_prefix_mla launch");
   if (p.slots > 0)
-    launch_pdl(prefix_mla_merge_kernel, dim3(unsigned(f.merge.tiles), DV / 8), dim3(BM), 0, stream,
+    launch_pdl(prefix_mla_merge_kernel, dim3(unsigned(f.merge.tiles) * BM), dim3(DV / 4), 0, stream,
                "shared_prefix_mla merge", a, f.merge, static_cast<const float*>(scratch),
                static_cast<const float*>(part_lse));
 }

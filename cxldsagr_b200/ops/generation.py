@@ -16,15 +16,6 @@ from . import reference
 from .native import lib
 
 
-def _records_ok(t: torch.Tensor) -> bool:
-    """Rows the kernels can load: contiguous records that start on 16-byte boundaries."""
-    if t.data_ptr() % 16:
-        return False
-    if t.numel() == 0:
-        return True
-    return t.stride(-1) == 1 and all(n == 1 or (s >= 0 and s % 8 == 0) for n, s in zip(t.shape[:-1], t.stride()))
-
-
 def shared_prefix_mla(q, prefix, tail, tail_lens, scale, *, return_lse: bool = False, value_dim: int = 512):
     """MLA of B continuations over one shared prefix and their own tails.
 
@@ -43,55 +34,30 @@ def shared_prefix_mla(q, prefix, tail, tail_lens, scale, *, return_lse: bool = F
     other parts of the attention.  On CUDA a length outside [0, S] is recorded
     in the device error word (``check_errors``) and clamped.
     """
-    if q.dim() not in (3, 4):
-        raise ValueError("q must be [B, H, D] or [B, T, H, D]")
     B, D = q.shape[0], q.shape[-1]
+    if q.dim() != 3 and q.dim() != 4:
+        raise ValueError("q must be [B, H, D] or [B, T, H, D]")
     if prefix.dim() != 2 or prefix.shape[1] != D:
         raise ValueError("prefix must be [P, D] with the query's record width")
     if tail is None:
         if tail_lens is not None:
             raise ValueError("tail_lens needs a tail")
-    elif tail.dim() != 3 or tail.shape[0] != B or tail.shape[2] != D:
-        raise ValueError("tail must be [B, S, D] with the query's batch and record width")
-    if tail_lens is not None and (tail_lens.dim() != 1 or tail_lens.shape[0] != B):
-        raise ValueError("tail_lens must be [B]")
-    if not (math.isfinite(scale) and scale > 0):
+    else:
+        if tail.dim() != 3 or tail.shape[0] != B or tail.shape[2] != D:
+            raise ValueError("tail must be [B, S, D] with the query's batch and record width")
+        if tail_lens is not None and tail_lens.shape != (B,):
+            raise ValueError("tail_lens must be [B]")
+    if not 0 < scale < math.inf:
         raise ValueError("scale must be positive and finite")
-    tensors = [t for t in (q, prefix, tail, tail_lens) if t is not None]
-    if any(t.device != q.device for t in tensors):
-        raise ValueError("q, prefix, tail and tail_lens must be on one device")
-    if not q.is_cuda:
+    if q.is_cuda:
+        if value_dim != 512:
+            raise ValueError("the sm_100a shared-prefix MLA kernel covers the V3.2 shape (576 / 512)")
+        out, lse = lib().shared_prefix_mla(q, prefix, tail, tail_lens, scale, return_lse)
+    else:
+        if any(t is not None and t.is_cuda for t in (prefix, tail, tail_lens)):
+            raise ValueError("q, prefix, tail and tail_lens must be on one device")
         out, lse = reference.shared_prefix_mla(q, prefix, tail, tail_lens, scale, value_dim)
-        return (out, lse) if return_lse else out
-    if value_dim != 512 or D != 576:
-        raise ValueError("the sm_100a shared-prefix MLA kernel covers the V3.2 shape (576 / 512)")
-    if any(t.dtype != torch.bfloat16 for t in (q, prefix) + (() if tail is None else (tail,))):
-        raise ValueError("q, prefix and tail must be BF16")
-    for name, t in (("prefix", prefix), ("tail", tail)):
-        if t is not None and not _records_ok(t):
-            raise ValueError(f"{name} records must be contiguous and start on 16-byte boundaries")
-    if tail_lens is not None and tail_lens.dtype != torch.int32:
-        raise ValueError("tail_lens must be int32")
-    q4 = (q if q.dim() == 4 else q.unsqueeze(1)).contiguous()
-    out = torch.empty((*q4.shape[:3], 512), dtype=torch.bfloat16, device=q.device)
-    lse = torch.empty(q4.shape[:3], dtype=torch.float32, device=q.device) if return_lse else None
-    lib().shared_prefix_mla(q4, prefix, tail, None if tail_lens is None else tail_lens.contiguous(), float(scale), out,
-                            lse)
-    out = out.view(*q.shape[:-1], 512)
-    return (out, lse.view(q.shape[:-1])) if return_lse else out
-
-
-def _sample_param(name, value, R, dtype, device, ok):
-    """(per-row tensor or None, scalar) of a sampling parameter; scalars are checked, device values are not."""
-    if torch.is_tensor(value):
-        if value.dim() != 1 or value.shape[0] != R or value.device != device:
-            raise ValueError(f"{name} must be a number or an [R] tensor on the logits' device")
-        if value.dtype != dtype:
-            raise ValueError(f"a per-row {name} must be {dtype}")
-        return value.contiguous(), 0
-    if not ok(value):
-        raise ValueError(f"{name} out of range: {value!r}")
-    return None, value
+    return (out, lse) if return_lse else out
 
 
 def sample_tokens(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
@@ -119,25 +85,29 @@ def sample_tokens(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError("logits must be [R, V] with V >= 1")
-    if logits.dtype not in (torch.float32, torch.bfloat16):
+    if logits.dtype is not torch.float32 and logits.dtype is not torch.bfloat16:
         raise ValueError("logits must be FP32 or BF16")
-    R = logits.shape[0]
-    dev = logits.device
-    if u.dim() != 1 or u.shape[0] != R or u.device != dev or u.dtype != torch.float32:
-        raise ValueError("u must be an FP32 [R] tensor on the logits' device")
-    t_t, t_0 = _sample_param("temperature", temperature, R, torch.float32, dev, lambda v: 0 <= v < math.inf)
-    k_t, k_0 = _sample_param("top_k", top_k, R, torch.int32, dev, lambda v: isinstance(v, int) and v >= 0)
-    p_t, p_0 = _sample_param("top_p", top_p, R, torch.float32, dev, lambda v: 0 <= v <= 1)
-    m_t, m_0 = _sample_param("min_p", min_p, R, torch.float32, dev, lambda v: 0 <= v <= 1)
+    tensor = torch.Tensor
+    if not isinstance(temperature, tensor) and not 0 <= temperature < math.inf:
+        raise ValueError(f"temperature out of range: {temperature!r}")
+    if not isinstance(top_k, tensor) and not (isinstance(top_k, int) and top_k >= 0):
+        raise ValueError(f"top_k must be a whole number, 0 or more: {top_k!r}")
+    if not isinstance(top_p, tensor) and not 0 <= top_p <= 1:
+        raise ValueError(f"top_p out of range: {top_p!r}")
+    if not isinstance(min_p, tensor) and not 0 <= min_p <= 1:
+        raise ValueError(f"min_p out of range: {min_p!r}")
     if not logits.is_cuda:
-        return reference.sample_tokens(logits, u, t_0 if t_t is None else t_t, k_0 if k_t is None else k_t,
-                                       p_0 if p_t is None else p_t, m_0 if m_t is None else m_t)
-    if logits.shape[1] > lib().sample_max_vocabulary():
-        raise ValueError(f"the sampling kernel takes vocabularies of up to {lib().sample_max_vocabulary()}")
-    if logits.stride(1) != 1 and logits.shape[1] > 1:
-        logits = logits.contiguous()
-    tokens = torch.empty(R, dtype=torch.int64, device=dev)
-    logprobs = torch.empty(R, dtype=torch.float32, device=dev)
-    lib().sample_tokens(logits, u.contiguous(), t_t, k_t, p_t, m_t, float(t_0), min(int(k_0), 2**31 - 1), float(p_0),
-                        float(m_0), tokens, logprobs)
-    return tokens, logprobs
+        R = logits.shape[0]
+        for name, v, dtype in (("u", u, torch.float32), ("temperature", temperature, torch.float32),
+                               ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
+                               ("min_p", min_p, torch.float32)):
+            if isinstance(v, tensor) and (v.shape != (R,) or v.dtype is not dtype or v.is_cuda):
+                raise ValueError(f"{name} must be a number or an [R] {dtype} tensor on the logits' device")
+        return reference.sample_tokens(logits, u, temperature, top_k, top_p, min_p)
+    t = temperature if isinstance(temperature, tensor) else None
+    k = top_k if isinstance(top_k, tensor) else None
+    p = top_p if isinstance(top_p, tensor) else None
+    m = min_p if isinstance(min_p, tensor) else None
+    return lib().sample_tokens(logits, u, t, k, p, m, 0.0 if t is not None else temperature,
+                               0 if k is not None else top_k, 0.0 if p is not None else top_p,
+                               0.0 if m is not None else min_p)
