@@ -998,6 +998,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("topk", &topk);
   m.def("sparse_mla", &sparse_mla);
   m.def("shared_prefix_mla", &shared_prefix_mla);
+  m.def("shared_prefix_mla_launches", [](int64_t B, int64_t T, int64_t H, int64_t P, int64_t S) {
+    b200::PrefixMLAArgs a{};
+    a.B = B; a.T = T; a.H = H; a.P = P; a.S = S;
+    return b200::shared_prefix_mla_launches(a);
+  });
   m.def("sample_tokens", &sample_tokens);
   m.def("sample_max_vocabulary", &b200::sample_max_vocabulary);
   m.def("sparse_mla_scratch_bytes", &sparse_mla_scratch_bytes);

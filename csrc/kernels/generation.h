@@ -41,6 +41,9 @@ struct PrefixMLAArgs {
 void launch_shared_prefix_mla(const PrefixMLAArgs& a, const std::function<float*(size_t)>& workspace,
                               cudaStream_t stream);
 
+// Kernels that a call of these sizes launches (0, 1, or 2 with the merge of partials).
+int shared_prefix_mla_launches(const PrefixMLAArgs& a);
+
 // ---------------------------------------------------------------- sampling
 struct SampleArgs {
   const void* logits;  // [R, V] FP32 or BF16, rows ld elements apart

@@ -832,6 +832,13 @@ void make_plan(const PrefixMLAArgs& a, FullPlan& f) {
 
 }  // namespace
 
+int shared_prefix_mla_launches(const PrefixMLAArgs& a) {
+  if (int64_t(a.B) * a.T * a.H == 0) return 0;
+  FullPlan f;
+  make_plan(a, f);
+  return f.plan.slots ? 2 : 1;
+}
+
 void launch_shared_prefix_mla(const PrefixMLAArgs& a, const std::function<float*(size_t)>& workspace,
                               cudaStream_t stream) {
   const int64_t rows = int64_t(a.B) * a.T * a.H;

@@ -45,6 +45,18 @@ class LayerState:
         return self.kv
 
 
+class TailState:
+    """One layer of a step of several continuations: the shared history records and the continuations' tails.
+
+    ``prefix`` [P, width]; ``tail`` [n, max, width], of which ``visible`` rows
+    (this step's included) count; ``rows``: where this step's records go, as
+    rows of ``tail`` seen as [n * max, width]; ``packed``: FP8 record scratch.
+    """
+
+    def __init__(self, prefix, tail, visible: int, rows, packed=None):
+        self.prefix, self.tail, self.visible, self.rows, self.packed = prefix, tail, visible, rows, packed
+
+
 class AttentionRunner:
     """Stateless w.r.t. requests: every call gets the session's :class:`LayerState`."""
 
@@ -142,6 +154,8 @@ class AttentionRunner:
                 logits_buf=None, comm=None, rows=None):
         """One chunk of attention; returns o_proj output for this rank's query rows."""
         scope = scope or (lambda _name: nullcontext())
+        if isinstance(state, TailState):
+            return self._continue(state, normed, quantized, positions, freqs, scope)
         cfg = self.cfg
         T_loc = normed.shape[0]
         T = positions.shape[0]
@@ -244,6 +258,35 @@ class AttentionRunner:
                 else:
                     attn = self._consume(cache, q_proj, ids)
         return self._output(attn, T_loc, scope)
+
+    def _continue(self, state: TailState, normed, quantized, positions, freqs, scope):
+        """One token of each continuation: every record of the shared history and of the own tail is
+        attended to, so the indexer and its selection are not needed."""
+        cfg, w = self.cfg, self.w
+        n = normed.shape[0]
+        H, nope, rope, L = cfg.n_heads, cfg.qk_nope_head_dim, cfg.qk_rope_head_dim, cfg.kv_lora_rank
+        with scope("attention_projection"):
+            with scope("fused_a_gemm"):
+                a = w.fused_a(normed, quantized=quantized)
+            qa = a[:, self.qa0:self.qa0 + self.qa_n]
+            with scope("kv_record"):
+                ops.kv_finish(a[:, self.kv0:self.kv0 + self.kv_n], L, rope, w.kv_norm, cfg.norm_eps, freqs, positions,
+                              state.tail.view(-1, state.tail.shape[-1]), state.rows, packed=state.packed)
+            with scope("q_norm"):
+                qa_normed, _, qr8, qrs = ops.norm_quant(qa, None, w.q_norm, cfg.norm_eps,
+                                                        want_out=w.fused_b.scales is None)
+            with scope("fused_b_gemm"):
+                b = w.fused_b(qa_normed, quantized=(qr8, qrs))
+            q_proj = torch.empty((n, H, cfg.qk_head_dim), dtype=torch.bfloat16, device=normed.device)
+            with scope("absorb"):
+                ops.mla_absorb(b, H, nope, rope, w.wk_b_t, q_proj)
+            with scope("q_rope"):
+                ops.mla_q_rope(b, H, nope, rope, freqs, positions, q_proj, L)
+        with scope("shared_prefix_mla"):
+            attn = ops.shared_prefix_mla(q_proj, state.prefix, state.tail[:, : state.visible], None,
+                                         cfg.attention_scale, value_dim=L)
+        self._prefetch_done = None
+        return self._output(attn, n, scope)
 
     def _cp_select(self, comm, q_idx, weights, keys, kscales, pos: int, end: int, T: int, r0: int, r1: int):
         """Exact top-k of this rank's query rows [r0, r1) with the indexer split by keys.

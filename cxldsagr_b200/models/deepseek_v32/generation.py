@@ -1,0 +1,137 @@
+"""Several continuations of one committed history, drawn token by token.
+
+The continuations of a request share its history: every layer attends to the
+session's committed records once for all of them (:func:`ops.shared_prefix_mla`)
+and to each continuation's own tail records, which live in a small buffer next
+to the session.  The session itself is not changed: no step is opened, nothing
+is appended, so a request can draw continuations, compare them and commit one
+with ``model.extend``.
+
+Attention here covers every visible record.  That equals the model's sparse
+attention while history and tail together fit the indexer's selection
+(``cfg.index_topk`` records); past that it is a different, dense attention, and
+has to be asked for with ``dense=True``.
+"""
+
+from __future__ import annotations
+
+from contextlib import nullcontext
+from dataclasses import dataclass
+
+import torch
+
+from ... import ops
+from .attention import TailState
+
+
+@dataclass
+class GenerationResult:
+    tokens: torch.Tensor     # int64 [n, steps]
+    logprobs: torch.Tensor   # fp32 [n, steps], each under the filtered distribution it was drawn from
+    lengths: torch.Tensor    # int64 [n]: tokens up to and including the first stop token
+
+
+class Continuations:
+    """``n`` continuations of ``session``'s committed history, at most ``max_tokens`` each.
+
+    :meth:`step` feeds one token per continuation and returns the logits of the
+    next one.  The records of the fed tokens are kept in ``tails`` (per layer
+    [n, max_tokens, 576]).
+    """
+
+    def __init__(self, model, n: int, max_tokens: int, *, session=None, dense: bool = False):
+        session = session or model.session
+        if n < 1 or max_tokens < 1:
+            raise ValueError("n and max_tokens must be positive")
+        if model.poisoned or session.failed or session.released:
+            raise RuntimeError("the session cannot be continued after a failure or release")
+        if model.cache_cfg.method != "hbm":
+            raise ValueError("continuations need the resident history of the hbm cache method")
+        if model.par.world > 1 or len(model.pool_devices) > 1 or model.replay_layout is not None:
+            raise ValueError("continuations run on one device, without a process group, placement or replay")
+        start = session.length
+        if start < 1:
+            raise ValueError("the session has no committed history")
+        cfg = model.cfg
+        if start + max_tokens > cfg.index_topk and not dense:
+            raise ValueError(f"history and continuation exceed the indexer's selection ({cfg.index_topk} records): "
+                             "attending to all of them differs from the model's sparse attention (dense=True allows it)")
+        if start + max_tokens > cfg.max_seq_len:
+            raise ValueError("history and continuation exceed the model's context")
+        self.model, self.session, self.start = model, session, start
+        self.n, self.max_tokens, self.length = n, max_tokens, 0
+        dev = model.device
+        self.tails = [torch.zeros((n, max_tokens, cfg.qk_head_dim), dtype=layer.kv.records.dtype, device=dev)
+                      for layer in session.layers]
+        self._first_rows = torch.arange(n, device=dev) * max_tokens
+        # FP8 caches: the records of a step pass through the packed form, as an appended chunk's do.
+        fp8 = session.layers[0].kv if session.layers[0].kv.kv_format == "fp8" else None
+        self._packed = None if fp8 is None else fp8.packed_rows(n)
+
+    def step(self, ids: torch.Tensor) -> torch.Tensor:
+        """Feed token ``ids[i]`` to continuation i; returns FP32 logits [n, vocab] of the token after it."""
+        model, cfg = self.model, self.model.cfg
+        if self.session.length != self.start or self.session.failed or self.session.released:
+            raise RuntimeError("the session's history changed since the continuations were opened")
+        if self.length == self.max_tokens:
+            raise ValueError("the continuations are full")
+        ids = ids.to(model.device).reshape(-1)
+        if ids.numel() != self.n:
+            raise ValueError("one token per continuation")
+        scope = model._scope()
+        t = self.length
+        positions = torch.full((self.n,), float(self.start + t), dtype=torch.float32, device=model.device)
+        rows = self._first_rows + t
+        with scope("embedding"):
+            hidden = ops.embed(ids, model.embed_table)
+        residual = None
+        for block, layer, tail in zip(model.blocks, self.session.layers, self.tails):
+            state = TailState(layer.kv.records[: self.start], tail, t + 1, rows, self._packed)
+            hidden, residual = block.forward(state, hidden, residual, self.start + t, positions, model.freqs, scope=scope)
+        with scope("final_norm_lm_head"):
+            normed, _ = ops.residual_rms_norm(hidden, residual, model.final_norm, cfg.norm_eps)
+            logits = model._lm_head(normed) if normed.is_cuda else ops.linear(normed, model.lm_head).float()
+        self.length = t + 1
+        return logits
+
+
+def generate(model, first_logits, n: int, max_tokens: int, *, session=None, temperature=1.0, top_k=0, top_p=1.0,
+             min_p=0.0, stop_token: int | None = None, generator: torch.Generator | None = None, uniforms=None,
+             dense: bool = False, scope=None) -> GenerationResult:
+    """Draw ``n`` continuations of up to ``max_tokens`` tokens after ``session``'s committed history.
+
+    ``first_logits`` [1, vocab] are the logits of the history's last token (what
+    ``model.prefill`` / ``extend`` returned).  Sampling parameters as in
+    :func:`ops.sample_tokens` (numbers, or tensors with one value per continuation);
+    the random numbers are ``uniforms`` [max_tokens, n] or drawn from
+    ``generator``.  A continuation that has drawn ``stop_token`` repeats it.
+    """
+    scope = scope or model.scope or (lambda _n: nullcontext())
+    dev = first_logits.device
+    if first_logits.dim() != 2 or first_logits.shape[0] != 1:
+        raise ValueError("first_logits must be the [1, vocab] logits of the history's last token")
+    if uniforms is None:
+        uniforms = torch.rand((max_tokens, n), generator=generator, device=dev)
+    elif uniforms.shape != (max_tokens, n):
+        raise ValueError("uniforms must be [max_tokens, n]")
+    # The last drawn token is not fed, so the tails hold max_tokens - 1 records.
+    run = Continuations(model, n, max_tokens - 1, session=session, dense=dense) if max_tokens > 1 else None
+    tokens = torch.empty((n, max_tokens), dtype=torch.int64, device=dev)
+    logprobs = torch.empty((n, max_tokens), dtype=torch.float32, device=dev)
+    lengths = torch.full((n,), max_tokens, dtype=torch.int64, device=dev)
+    done = torch.zeros(n, dtype=torch.bool, device=dev)
+    logits = first_logits.expand(n, -1)
+    for t in range(max_tokens):
+        with scope("sample"):
+            drawn, lp = ops.sample_tokens(logits, uniforms[t], temperature=temperature, top_k=top_k, top_p=top_p,
+                                          min_p=min_p)
+        if stop_token is not None:
+            drawn = torch.where(done, stop_token, drawn)
+            lp = torch.where(done, 0.0, lp)
+            stops = (drawn == stop_token) & ~done
+            lengths = torch.where(stops, t + 1, lengths)
+            done |= stops
+        tokens[:, t], logprobs[:, t] = drawn, lp
+        if t + 1 < max_tokens:
+            logits = run.step(drawn)
+    return GenerationResult(tokens, logprobs, lengths)

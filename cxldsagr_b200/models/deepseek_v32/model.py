@@ -701,6 +701,12 @@ class DeepSeekV32Model:
     def candidate(self, ids, *, session: ModelSession | None = None):
         return self.forward(ids, session=session, transient=True)
 
+    def generate(self, first_logits, n: int, max_tokens: int, **kw):
+        """Draw ``n`` continuations of the committed history (see :func:`.generation.generate`)."""
+        from .generation import generate
+
+        return generate(self, first_logits, n, max_tokens, **kw)
+
     def truncate(self, length: int, *, session: ModelSession | None = None):
         (session or self.session).truncate(length)
 

@@ -27,8 +27,16 @@ def _fp8_gemm_launches(mod, args):
     q, w = args[0], args[2]
     ue8m0 = bool(args[6]) if len(args) > 6 else False
     return 2 if mod.fp8_gemm_splits(q.shape[0], w.shape[0], q.shape[1], ue8m0) > 1 else 1  # + split-K reduce
+
+
+def _shared_prefix_mla_launches(mod, args):
+    q, prefix, tail = args[:3]
+    T = q.shape[1] if q.dim() == 4 else 1
+    return mod.shared_prefix_mla_launches(q.shape[0], T, q.shape[-2], prefix.shape[0], 0 if tail is None else tail.shape[1])
+
+
 _NO_LAUNCH = {"error_word", "sparse_mla_scratch_bytes", "fp8_gemm_splits", "set_decode_gemv", "set_gemv_k_split", "set_pdl",
-              "pdl_enabled", "sample_max_vocabulary"}
+              "pdl_enabled", "sample_max_vocabulary", "shared_prefix_mla_launches"}
 
 
 class _CountingLib:
@@ -49,6 +57,8 @@ class _CountingLib:
         multi = _MULTI_LAUNCH.get(name)
         if name == "fp8_gemm":
             multi = lambda args: _fp8_gemm_launches(self._mod, args)  # noqa: E731
+        elif name == "shared_prefix_mla":
+            multi = lambda args: _shared_prefix_mla_launches(self._mod, args)  # noqa: E731  (+ merge of partials)
 
         def call(*args, **kwargs):
             self.launches += multi(args) if multi else 1

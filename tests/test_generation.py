@@ -1,0 +1,175 @@
+"""Drawing several continuations of one committed history through the model."""
+
+import json
+import math
+
+import pytest
+import torch
+
+from cxldsagr_b200 import ops
+from cxldsagr_b200.checkpoint import StateDictSource, random_state_dict
+from cxldsagr_b200.config import CacheConfig, tiny_config, v32_config
+from cxldsagr_b200.models.deepseek_v32.generation import Continuations
+from cxldsagr_b200.models.deepseek_v32.model import DeepSeekV32Model
+
+HIST = 40
+
+
+@pytest.fixture(scope="module")
+def tiny():
+    cfg = tiny_config()
+    return cfg, StateDictSource(random_state_dict(cfg, seed=0))
+
+
+def make(cfg, src, device="cpu", capacity=128, **kw):
+    return DeepSeekV32Model(cfg, src, device=device, cache=CacheConfig(capacity=capacity, chunk_size=64, **kw))
+
+
+def history(cfg, n=HIST, seed=0):
+    return torch.randint(0, cfg.vocab_size, (n,), generator=torch.Generator().manual_seed(seed))
+
+
+@pytest.mark.parametrize("kv_format", ["bf16", "fp8"])
+def test_steps_equal_extends(tiny, kv_format):
+    """Feeding the same tokens one by one gives each continuation the logits of its own extended history."""
+    cfg, src = tiny
+    hist = history(cfg)
+    paths = torch.randint(0, cfg.vocab_size, (3, 4), generator=torch.Generator().manual_seed(1))
+    m = make(cfg, src, kv_format=kv_format)
+    m.prefill(hist)
+    run = Continuations(m, 3, 4)
+    got = torch.stack([run.step(paths[:, t]) for t in range(4)], 1)
+    for i in range(3):
+        m.reset()
+        m.prefill(hist)
+        for t in range(4):
+            want = m.extend(paths[i, t:t + 1]).logits[0]
+            # The same oracles on the same records; only the row count of the linears differs.
+            assert (got[i, t] - want).abs().max() <= 2.0**-6 * want.abs().max()
+
+
+def test_greedy_generation_follows_the_extends(tiny):
+    cfg, src = tiny
+    hist = history(cfg, seed=2)
+    m = make(cfg, src)
+    first = m.prefill(hist).logits
+    out = m.generate(first, 2, 6, temperature=0.0)
+    assert out.tokens.shape == (2, 6) and torch.equal(out.tokens[0], out.tokens[1])
+    assert not out.logprobs.abs().any()
+    logits, want = first, []
+    for _ in range(6):
+        want.append(int(logits.argmax(-1)))
+        logits = m.extend(torch.tensor([want[-1]])).logits
+    assert out.tokens[0].tolist() == want
+
+
+def test_session_is_untouched_and_draws_are_repeatable(tiny):
+    cfg, src = tiny
+    hist, ext = history(cfg, seed=3), history(cfg, 3, seed=4)
+    m = make(cfg, src)
+    first = m.prefill(hist).logits
+    plain = m.extend(ext).logits
+    m.reset()
+    first = m.prefill(hist).logits
+    records = [layer.kv.records.clone() for layer in m.session.layers]
+    u = torch.rand(5, 4, generator=torch.Generator().manual_seed(5))
+    a = m.generate(first, 4, 5, uniforms=u, temperature=1.5, top_k=50)
+    assert m.length == HIST and all(c.length == HIST for c in m.caches)
+    assert all(torch.equal(layer.kv.records, r) for layer, r in zip(m.session.layers, records))
+    b = m.generate(first, 4, 5, uniforms=u, temperature=1.5, top_k=50)
+    assert torch.equal(a.tokens, b.tokens) and torch.equal(a.logprobs, b.logprobs)
+    one = m.generate(first, 1, 5, uniforms=u[:, 2:3], temperature=1.5, top_k=50)
+    assert torch.equal(one.tokens[0], a.tokens[2])
+    assert torch.equal(m.extend(ext).logits, plain)
+
+
+def test_stop_token_and_lengths(tiny):
+    cfg, src = tiny
+    m = make(cfg, src)
+    first = m.prefill(history(cfg, seed=6)).logits
+    u = torch.rand(6, 3, generator=torch.Generator().manual_seed(7))
+    free = m.generate(first, 3, 6, uniforms=u, temperature=2.0)
+    stop = int(free.tokens[1, 2])
+    out = m.generate(first, 3, 6, uniforms=u, temperature=2.0, stop_token=stop)
+    at = free.tokens[1].tolist().index(stop)
+    assert int(out.lengths[1]) == at + 1
+    assert torch.equal(out.tokens[1, : at + 1], free.tokens[1, : at + 1])
+    assert (out.tokens[1, at:] == stop).all() and not out.logprobs[1, at + 1:].any()
+
+
+def test_refusals(tiny):
+    cfg, src = tiny
+    m = make(cfg, src)
+    with pytest.raises(ValueError, match="no committed history"):
+        Continuations(m, 1, 1)
+    first = m.prefill(history(cfg)).logits
+    for bad in (lambda: Continuations(m, 0, 1), lambda: Continuations(m, 1, 0),
+                lambda: Continuations(m, 1, cfg.index_topk - HIST + 1),
+                lambda: m.generate(first.expand(2, -1), 1, 2),
+                lambda: m.generate(first, 2, 2, uniforms=torch.rand(2, 3)),
+                lambda: m.generate(first, 2, 2, temperature=-1.0)):
+        with pytest.raises(ValueError):
+            bad()
+    dense = Continuations(m, 1, cfg.index_topk, dense=True)
+    dense.step(torch.tensor([1]))
+    run = Continuations(m, 2, 1)
+    with pytest.raises(ValueError, match="one token"):
+        run.step(torch.tensor([1]))
+    run.step(torch.tensor([1, 2]))
+    with pytest.raises(ValueError, match="full"):
+        run.step(torch.tensor([1, 2]))
+    m.extend(torch.tensor([3]))
+    with pytest.raises(RuntimeError, match="changed"):
+        dense.step(torch.tensor([1]))
+    off = make(cfg, src, method="serial_sparse", pool_tokens=128, host_tokens=128)
+    off.prefill(history(cfg))
+    with pytest.raises(ValueError, match="hbm"):
+        Continuations(off, 1, 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layers,hist,n", [([0], 700, 5), ([0, 3], 130, 9)])
+def test_v32_steps_match_extends_on_gpu(layers, hist, n):
+    """V3.2 dimensions (a dense layer; a dense and a mixture-of-experts layer): shared-prefix attention against
+    the sparse path with every record selected."""
+    dev = "cuda"
+    cfg = v32_config(4 if 3 in layers else 1, n_routed_experts=16, n_group=4, topk_group=2) if 3 in layers else v32_config(1)
+    src = StateDictSource(random_state_dict(cfg, layers=layers, seed=1, device=dev))
+    m = DeepSeekV32Model(cfg, src, device=dev, layers=layers, cache=CacheConfig(capacity=1024, chunk_size=512))
+    ids = history(cfg, hist).to(dev)
+    paths = history(cfg, 3 * n, seed=2).reshape(n, 3).to(dev)
+    first = m.prefill(ids).logits
+    run = Continuations(m, n, 3)
+    got = torch.stack([run.step(paths[:, t]) for t in range(3)], 1)
+    ops.check_errors(dev)
+    for i in (0, n - 1):
+        m.reset()
+        m.prefill(ids)
+        for t in range(3):
+            want = m.extend(paths[i, t:t + 1]).logits[0]
+            # BF16 activations through other tile shapes (2^-8 per rounding, a dozen roundings per layer).
+            assert (got[i, t] - want).abs().max() <= 2.0**-4 * want.abs().max()
+    out = m.generate(first, n, 4, temperature=0.8, top_k=100, top_p=0.95, session=_fresh(m, ids))
+    ops.check_errors(dev)
+    assert ((out.tokens >= 0) & (out.tokens < cfg.vocab_size)).all()
+    assert torch.isfinite(out.logprobs).all() and (out.logprobs <= 0).all()
+
+
+def _fresh(m, ids):
+    m.reset()
+    m.prefill(ids)
+    return m.session
+
+
+@pytest.mark.gpu
+def test_infer_cli_draws_continuations(tmp_path, capsys):
+    from cxldsagr_b200.models.deepseek_v32 import infer
+
+    path = tmp_path / "ids.json"
+    path.write_text(json.dumps(history(v32_config(1), 300).tolist()))
+    infer.main(["--random-init", "--num-layers", "1", "--input-ids", str(path), "--history", "290", "--samples", "3",
+                "--new-tokens", "4", "--temperature", "0.7", "--top-p", "0.9", "--seed", "1"])
+    answer = json.loads(capsys.readouterr().out.strip().splitlines()[-1])
+    assert answer["length"] == 300 and len(answer["continuations"]) == 3
+    assert all(len(c) == 4 for c in answer["continuations"])
+    assert all(p <= 0 and math.isfinite(p) for row in answer["logprobs"] for p in row)

@@ -488,3 +488,24 @@ def test_sample_refusals():
     tok, lp = ops.sample_tokens(x[:0], u[:0])
     assert tok.shape == (0,) and lp.shape == (0,)
     assert ref.SAMPLE_FIXED == FIXED
+
+
+@gpu
+def test_launch_counts():
+    """The launch counter counts the merge of partials where a call has one."""
+    from cxldsagr_b200.ops.native import launch_count
+
+    def launches(B, T, H, P, S):
+        q, prefix, tail = prefix_inputs(B, T, H, P, S, "cuda")
+        n = launch_count()
+        ops.shared_prefix_mla(q, prefix, tail, None, SCALE)
+        return launch_count() - n
+
+    assert launches(2, 1, 128, 64, 1) == 1
+    assert launches(1, 1, 128, 20000, 1) == 2
+    assert launches(3, 1, 16, 64, 2) == 2  # heads that do not fill a tile: tails are merged in
+    assert launches(0, 1, 128, 64, 1) == 0
+    x, u = rows(2, 100)
+    n = launch_count()
+    ops.sample_tokens(x, u)
+    assert launch_count() - n == 1
