@@ -17,7 +17,7 @@
 //
 // A row belongs to a cluster of 1 to 16 CTAs: it is read from HBM once and
 // stays in their shared memory for all later passes (first as logits, then as
-// d).  The CTAs exchange values through distributed shared memory.  Nothing
+// d); with many long rows, one CTA per row reads it again instead.  The CTAs exchange values through distributed shared memory.  Nothing
 // spins: they meet at hardware barriers only (six per row with one filter, two without).
 #include <algorithm>
 #include <cmath>
@@ -126,8 +126,9 @@ __device__ __forceinline__ uint64_t warp_inclusive64(uint64_t v) {
 // A row as one CTA of its cluster sees it.  Positions [0, chunk * kWarps) cover
 // the CTA's slice of the row (index = begin + position) with some padding;
 // warp w owns [w * chunk, + chunk).  NaN logits and padding turn into a d that
-// no comparison accepts.
-template <bool BF16>
+// no comparison accepts.  RESIDENT: the slice stays in shared memory, otherwise
+// every pass reads it again.
+template <bool BF16, bool RESIDENT>
 struct Row {
   Shared& s;
   float* v;                // logits, then d
@@ -136,6 +137,7 @@ struct Row {
   int begin, start, stop;  // index of position 0; the slice's entries are [start, stop)
   int w0, w1, sub;         // this warp's positions, in parts of `sub`
   float mx, T, inv, scale; // scale: a power of two applied to logit differences and T, 1 for usual rows
+  bool usual;              // no scaling
   int phase = 0, turn = 0, event = 0, gathers = 0;  // buffers in use
 
   __device__ Row(Shared& s_) : s(s_) {}
@@ -157,27 +159,70 @@ struct Row {
     const float q = a * inv;
     return fmaf(fmaf(-q, T, a), inv, q);
   }
-  __device__ float dist(float x) const { return quotient(x == mx ? 0.f : (x - mx) * scale); }
+  __device__ float dist(float x) const {
+    return x > -INFINITY ? quotient(x == mx ? 0.f : (x - mx) * scale) : -INFINITY;
+  }
   __device__ static float weight(float d) { return expf(d); }
 
-  // f(j, d) for four positions per lane and step.
-  template <typename F>
-  __device__ void sweep(int j0, int j1, F&& f) const {
-    for (int j = j0 + 4 * int(threadIdx.x % 32); j < j1; j += kStep) {
-      const float4 q = quad(j);
-      const float d[4] = {q.x, q.y, q.z, q.w};
-      f(j, d);
+  // Four logits of a streamed row.
+  __device__ float4 load4(int j) const {
+    const int i = begin + j;
+    if (i >= start && i + 4 <= stop) {
+      if constexpr (BF16) {
+        const uint2 q = __ldg(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(src) + i));
+        return make_float4(bf16_lo(q.x), bf16_hi(q.x), bf16_lo(q.y), bf16_hi(q.y));
+      } else {
+        return __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(src) + i));
+      }
+    }
+    return make_float4(at(j), at(j + 1), at(j + 2), at(j + 3));
+  }
+  __device__ void dist4(const float4& q, float (&d)[4]) const {
+    if (usual) {
+      d[0] = quotient(q.x - mx);
+      d[1] = quotient(q.y - mx);
+      d[2] = quotient(q.z - mx);
+      d[3] = quotient(q.w - mx);
+    } else {
+      d[0] = dist(q.x);
+      d[1] = dist(q.y);
+      d[2] = dist(q.z);
+      d[3] = dist(q.w);
     }
   }
-  // The same while the logits are replaced by their distances (base: the best logit, 0 in a scaled row).
+  // f(j, x) for four positions per lane and step: logits (at first), d once a resident row holds it.
   template <typename F>
-  __device__ void first_sweep(int j0, int j1, float base, F&& f) {
-    for (int j = j0 + 4 * int(threadIdx.x % 32); j < j1; j += kStep) {
-      const float4 q = quad(j);
-      const float d[4] = {quotient(q.x - base), quotient(q.y - base), quotient(q.z - base), quotient(q.w - base)};
-      quad(j) = make_float4(d[0], d[1], d[2], d[3]);
-      f(j, d);
+  __device__ void raw_sweep(int j0, int j1, F&& f) const {
+    int j = j0 + 4 * int(threadIdx.x % 32);
+    if constexpr (RESIDENT) {
+      for (; j < j1; j += kStep) f(j, quad(j));
+    } else {  // the next two steps' loads are in flight
+      float4 n0 = load4(j), n1 = load4(j + kStep);
+      for (; j < j1; j += kStep) {
+        const float4 q = n0;
+        n0 = n1;
+        n1 = load4(j + 2 * kStep);
+        f(j, q);
+      }
     }
+  }
+  template <typename F>
+  __device__ void sweep(int j0, int j1, F&& f) const {
+    raw_sweep(j0, j1, [&](int j, const float4& q) {
+      float d[4] = {q.x, q.y, q.z, q.w};
+      if constexpr (!RESIDENT) dist4(q, d);
+      f(j, d);
+    });
+  }
+  // The first sweep over d: a resident row's logits are replaced by it.
+  template <typename F>
+  __device__ void first_sweep(int j0, int j1, F&& f) {
+    raw_sweep(j0, j1, [&](int j, const float4& q) {
+      float d[4];
+      dist4(q, d);
+      if constexpr (RESIDENT) quad(j) = make_float4(d[0], d[1], d[2], d[3]);
+      f(j, d);
+    });
   }
 
   // ------------------------------------------------ the CTA and the cluster
@@ -229,16 +274,45 @@ struct Row {
     for (int b = threadIdx.x; b < kBins; b += kThreads) s.cnt[b] = s.lo[b] = s.hi[b] = 0;
     __syncthreads();
   }
-  // In halves of 18 bits: sums of 16,384 of them fit a word, and no addition waits for a carry.
+  // In halves of 18 bits: sums of 16,384 of them fit a word, and no addition waits for a carry.  (A streamed
+  // slice folds them into the threads' 64-bit sums every kSlice positions.)
   __device__ void add_mass(int b, uint64_t m) {
     atomicAdd(&s.hi[b], uint32_t(m >> 18));
     atomicAdd(&s.lo[b], uint32_t(m) & 0x3ffffu);
+  }
+  // Between rounds of a streamed slice (one CTA per row): into the row's histogram.
+  __device__ void fold(bool first) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int b = 2 * threadIdx.x + i;
+      const uint64_t m = (uint64_t(s.hi[b]) << 18) + s.lo[b];
+      s.all_cnt[b] = first ? s.cnt[b] : s.all_cnt[b] + s.cnt[b];
+      s.all_mass[b] = first ? m : s.all_mass[b] + m;
+      s.cnt[b] = s.lo[b] = s.hi[b] = 0;
+    }
+    __syncthreads();
+  }
+  // f(j0, j1) over this warp's positions, folding the histogram where its words could overflow.
+  template <typename F>
+  __device__ void rounds(F&& f) {
+    if constexpr (RESIDENT) {
+      f(w0, w1);
+    } else {
+      constexpr int kRound = kSlice / kWarps;
+      for (int j = w0; j < w1; j += kRound) {
+        f(j, min(w1, j + kRound));
+        fold(j == w0);
+      }
+    }
   }
   // CTA c sums the bins [c, c + 1) * kBins / C of all CTAs and hands them to all; every thread then holds
   // what lies before its two bins.
   __device__ void merge() {
     cluster_sync();
-    if (C == 1) {
+    if constexpr (!RESIDENT) {
+      // folded already
+    } else if (C == 1) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int b = 2 * threadIdx.x + i;
@@ -312,14 +386,36 @@ struct Row {
   template <typename F>
   __device__ void histogram(F&& entry) {
     clear_histogram();
-    for (int j = w0 + int(threadIdx.x % 32); j < w1; j += 32) {
-      int b;
-      float w;
-      if (entry(j, b, w)) {
-        atomicAdd(&s.cnt[b], 1u);
-        add_mass(b, mass_of(w));
+    rounds([&](int j0, int j1) {
+      for (int j = j0 + int(threadIdx.x % 32); j < j1; j += 32) {
+        int b;
+        float w;
+        if (entry(j, b, w)) {
+          atomicAdd(&s.cnt[b], 1u);
+          add_mass(b, mass_of(w));
+        }
       }
-    }
+    });
+    merge();
+  }
+
+  // The same with bins of d: bin(d) < 0 leaves an entry out.
+  template <typename F>
+  __device__ void histogram_of_d(F&& bin) {
+    clear_histogram();
+    rounds([&](int j0, int j1) {
+      sweep(j0, j1, [&](int, const float (&d)[4]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (d[e] > -kSpan) {
+            const int b = bin(d[e]);
+            if (b >= 0) {
+              atomicAdd(&s.cnt[b], 1u);
+              add_mass(b, mass_of(weight(d[e])));
+            }
+          }
+      });
+    });
     merge();
   }
 
@@ -558,13 +654,13 @@ struct Row {
   }
 };
 
-template <bool BF16>
+template <bool BF16, bool RESIDENT>
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_constant__ SampleArgs a, int C, int chunk) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   pdl_trigger();
   pdl_wait();
   Shared& s = *reinterpret_cast<Shared*>(smem_raw);
-  using R = Row<BF16>;
+  using R = Row<BF16, RESIDENT>;
   constexpr int VEC = BF16 ? 8 : 4;
   constexpr int kSize = BF16 ? 2 : 4;
   const int64_t row = blockIdx.x / C;
@@ -594,14 +690,19 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   r.stop = min(a.V, vec0 + per);
   r.begin = r.start - pad;
   float mx = -INFINITY, mn = INFINITY;  // mn: of some finite entries, for the histogram's range
-  if (r.rank == 0 && int(threadIdx.x) < pad + head)
-    r.v[threadIdx.x] = mx = int(threadIdx.x) < pad ? -INFINITY : r.logit(int(threadIdx.x) - pad);
+  if (r.rank == 0 && int(threadIdx.x) < pad + head) {
+    mx = int(threadIdx.x) < pad ? -INFINITY : r.logit(int(threadIdx.x) - pad);
+    if constexpr (RESIDENT) r.v[threadIdx.x] = mx;
+  }
   // NaN passes through: fmaxf and fminf ignore it.
   const int vecs = (r.stop - vec0) / VEC;
 #pragma unroll 4
   for (int g = threadIdx.x; g < vecs; g += kThreads) {
     const int i = vec0 + g * VEC, j = i - r.begin;
-    const uint4 raw = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(r.src) + int64_t(i) * kSize));
+    const uint4* at = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(r.src) + int64_t(i) * kSize);
+    uint4 raw;
+    if constexpr (RESIDENT) raw = __ldcs(at);
+    else raw = __ldg(at);
     float x[VEC];
     if constexpr (BF16) {
       const uint32_t q[4] = {raw.x, raw.y, raw.z, raw.w};
@@ -620,13 +721,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
 #pragma unroll
     for (int e = 0; e < VEC; e += 4) {
       mx = fmaxf(fmaxf(mx, fmaxf(x[e], x[e + 1])), fmaxf(x[e + 2], x[e + 3]));
-      r.quad(j + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+      if constexpr (RESIDENT) r.quad(j + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
     }
   }
   // The entries after the last whole vector, then the padding.
-  for (int j = vec0 + vecs * VEC - r.begin + int(threadIdx.x); j < chunk * kWarps; j += kThreads) {
+  for (int j = vec0 + vecs * VEC - r.begin + int(threadIdx.x); j < (RESIDENT ? chunk * kWarps : r.stop - r.begin);
+       j += kThreads) {
     const float x = r.begin + j < r.stop ? r.logit(r.begin + j) : -INFINITY;
-    r.v[j] = x;
+    if constexpr (RESIDENT) r.v[j] = x;
     mx = fmaxf(mx, x);
   }
   {
@@ -657,7 +759,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   }
   if (!(T > 0.f) || k == 1 || p <= 0.f || mp > 1.f) {  // only the best entry: the first of the equal ones
     uint64_t first = kNothing;
-    r.sweep(w0, w1, [&](int j, const float (&x)[4]) {
+    r.raw_sweep(w0, w1, [&](int j, const float4& q) {
+      const float x[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
       for (int e = 3; e >= 0; --e)
         if (x[e] == mx) first = min(first, uint64_t(r.begin + j + e));
@@ -671,19 +774,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     }
     return;
   }
-  float base = mx;
   r.T = T;
   r.scale = 1.f;
-  if (!(T > 0x1p-40f && T < 0x1p40f && mx < INFINITY)) {
+  r.usual = T > 0x1p-40f && T < 0x1p40f && mx < INFINITY;
+  if (!r.usual) {
     // An extreme temperature (or infinite logits): differences and T by a power of two, T towards 1.
     r.scale = T < INFINITY ? ldexpf(1.f, min(126, max(-126, -ilogbf(T)))) : 0.f;
     r.T = T < INFINITY ? T * r.scale : 1.f;
-    base = 0.f;
-    for (int j = w0 + lane; j < w1; j += 32) {
-      const float x = r.v[j];
-      r.v[j] = x == mx ? 0.f : x > -INFINITY ? (x - mx) * r.scale : -INFINITY;
-    }
-    __syncwarp();
   }
   r.inv = 1.f / r.T;
   const bool cut_k = k > 0 && k < a.V, cut_p = p < 1.f;
@@ -695,47 +792,32 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     const float bins = (kBins - 1) / range;
     auto bin_of = [&](float d) { return min(kBins - 1, __float_as_int(fmaf(-d, bins, 8388608.f)) - 0x4b000000); };
     r.clear_histogram();
-    if (cut_p)
-      r.first_sweep(w0, w1, base, [&](int, const float (&d)[4]) {
+    r.rounds([&](int j0, int j1) {
+      if (cut_p)
+        r.first_sweep(j0, j1, [&](int, const float (&d)[4]) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint64_t m = mass_of(R::weight(d[e]));
-          if (m) {
-            const int b = bin_of(d[e]);
-            if (cut_k) atomicAdd(&s.cnt[b], 1u);
-            r.add_mass(b, m);
+          for (int e = 0; e < 4; ++e) {
+            const uint64_t m = mass_of(R::weight(d[e]));
+            if (m) {
+              const int b = bin_of(d[e]);
+              if (cut_k) atomicAdd(&s.cnt[b], 1u);
+              r.add_mass(b, m);
+            }
           }
-        }
-      });
-    else
-      r.first_sweep(w0, w1, base, [&](int, const float (&d)[4]) {
+        });
+      else
+        r.first_sweep(j0, j1, [&](int, const float (&d)[4]) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (d[e] > -kSpan) atomicAdd(&s.cnt[bin_of(d[e])], 1u);
-      });
+          for (int e = 0; e < 4; ++e)
+            if (d[e] > -kSpan) atomicAdd(&s.cnt[bin_of(d[e])], 1u);
+        });
+    });
     r.merge();
-    auto rebuild = [&]() {  // after the histogram's memory was used
-      r.histogram([&](int j, int& b, float& w) {
-        const float d = r.v[j];
-        if (!(d > -kSpan)) return false;
-        b = bin_of(d);
-        w = R::weight(d);
-        return true;
-      });
-    };
     uint64_t through = r.total_mass;  // mass left by top-k
     typename R::Goal gk{false, uint64_t(k), 0.}, gp{true, 0, 0.};
     typename R::Cut ck{-1, 0, 0, 0, 0}, cp{-1, 0, 0, 0, 0};
     if (cut_k && uint64_t(k) < r.total_count) ck = r.find_bin(gk);
     bool k_done = ck.bin < 0;  // fewer entries with mass than k: no cut
-    auto slow = [&](const typename R::Cut& c, const typename R::Goal& g, uint64_t& t) {
-      return r.find_cut(
-          [&](float x) {
-            const float d = r.dist(x);
-            return d > -kSpan && bin_of(d) == c.bin;
-          },
-          c, g, t);
-    };
     typename R::Cut cq = cp;
     if (cut_p) {
       // Bounds of the mass left by top-k bound the bins in which top-p can cut.
@@ -749,45 +831,87 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         cq = r.find_bin(gp);
       }
     }
+    // The listed entries of this CTA that are kept after all.
+    auto add_listed = [&]() {
+      for (int e = threadIdx.x; e < int(s.own_count); e += kThreads) {
+        const uint64_t c = s.list[s.own_base + e].x;
+        if (c >= cut) {
+          const float w = R::weight(r.dist(key_value(uint32_t(c >> 32))));
+          const int j = s.own[e], part = j / chunk * kSubs + j % chunk / r.sub;
+          if (!(w < mp)) atomicAdd(reinterpret_cast<unsigned long long*>(&s.sub[part]), mass_of(w));
+        }
+      }
+      __syncthreads();
+      summed = true;
+    };
+    // One cut in a bin with many entries: 1,024 finer bins of it, then the list, or the keys' bits if even a
+    // finer bin does not fit (equal logits).
+    auto settle = [&](const typename R::Cut& c, const typename R::Goal& g, bool by_k) {
+      const float offset = 0.5f - float(c.bin);
+      auto fine = [&](float d) { return min(kBins - 1, max(0, int(fmaf(-d, bins, offset) * kBins))); };
+      r.histogram_of_d([&](float d) { return bin_of(d) == c.bin ? fine(d) : -1; });
+      const typename R::Cut f = r.find_bin(g, c.count, c.mass);
+      if (f.entries <= kList) {
+        const int n = r.gather(
+            [&](float d, bool& want) -> uint64_t {
+              const int b = bin_of(d);
+              if (b < c.bin || (b == c.bin && fine(d) < f.bin)) {
+                const float w = R::weight(d);
+                return mass_of(w < mp ? 0.f : w);
+              }
+              want = b == c.bin && fine(d) == f.bin && d > -kSpan;
+              return 0;
+            },
+            [&](float) { return by_k ? kInK : kInP; });
+        cut = max(cut, r.rank_list(n, by_k, gk, f, !by_k, p, f, through));
+        add_listed();
+      } else {
+        uint64_t unused;
+        cut = max(cut, r.find_cut(
+                           [&](float x) {
+                             const float d = r.dist(x);
+                             return d > -kSpan && bin_of(d) == c.bin && fine(d) == f.bin;
+                           },
+                           f, g, by_k ? through : unused));
+        summed = false;
+      }
+    };
     if (cut_p || !k_done) {
-      // One pass: entries before the first cut bin are kept for certain, those of the cut bins are listed.
-      const int kb = k_done ? -1 : ck.bin, p0 = cut_p ? cp.bin : kBins, p1 = cut_p ? cq.bin : -1;
-      const int sure = cut_p ? p0 : kb;
-      auto group = [&](int b) { return (b == kb ? kInK : 0ull) | (b >= p0 && b <= p1 ? kInP : 0ull); };
-      const int n = r.gather(
-          [&](float d, bool& want) -> uint64_t {
-            const int b = bin_of(d);
-            if (b < sure) {
-              const float w = R::weight(d);
-              return mass_of(w < mp ? 0.f : w);
-            }
-            want = (b == kb || (b >= p0 && b <= p1)) && d > -kSpan;
-            return 0;
-          },
-          [&](float x) { return group(bin_of(r.dist(x))); });
+      // How many entries would be listed; without counts, at most a bin's mass over that at its lower end.
+      auto at_most = [&](const typename R::Cut& c) {
+        return float(c.bin_mass) / (R::weight(-(float(c.bin) + 0.5f) / bins) * kFixed);
+      };
+      float listed = k_done ? 0.f : float(ck.entries);
+      if (cut_p) listed += cut_k ? float(cq.count + cq.entries - cp.count) : at_most(cp);
+      int n = kList + 1;
+      if (listed <= kList) {
+        // One pass: entries before the first cut bin are kept for certain, those of the cut bins are listed.
+        const int kb = k_done ? -1 : ck.bin, p0 = cut_p ? cp.bin : kBins, p1 = cut_p ? cq.bin : -1;
+        const int sure = cut_p ? p0 : kb;
+        auto group = [&](int b) { return (b == kb ? kInK : 0ull) | (b >= p0 && b <= p1 ? kInP : 0ull); };
+        n = r.gather(
+            [&](float d, bool& want) -> uint64_t {
+              const int b = bin_of(d);
+              if (b < sure) {
+                const float w = R::weight(d);
+                return mass_of(w < mp ? 0.f : w);
+              }
+              want = (b == kb || (b >= p0 && b <= p1)) && d > -kSpan;
+              return 0;
+            },
+            [&](float x) { return group(bin_of(r.dist(x))); });
+      }
       if (n <= kList) {
         cut = r.rank_list(n, !k_done, gk, ck, cut_p, p, cp, through);
-        // The listed entries of this CTA that are kept after all.
-        for (int e = threadIdx.x; e < int(s.own_count); e += kThreads) {
-          const uint64_t c = s.list[s.own_base + e].x;
-          if (c >= cut) {
-            const float w = R::weight(r.dist(key_value(uint32_t(c >> 32))));
-            const int j = s.own[e], part = j / chunk * kSubs + j % chunk / r.sub;
-            if (!(w < mp)) atomicAdd(reinterpret_cast<unsigned long long*>(&s.sub[part]), mass_of(w));
-          }
-        }
-        __syncthreads();
-        summed = true;
+        add_listed();
       } else {
         if (!k_done) {
-          cut = slow(ck, gk, through);
-          if (cut_p) rebuild();
+          settle(ck, gk, true);
+          if (cut_p) r.histogram_of_d(bin_of);
         }
         if (cut_p) {
           gp.want = double(p) * double(through);
-          cp = r.find_bin(gp);
-          uint64_t unused;
-          cut = max(cut, slow(cp, gp, unused));
+          settle(r.find_bin(gp), gp, false);
         }
       }
     }
@@ -816,7 +940,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
           for (int e = 0; e < 4; ++e) m += mass_of(kept_weight(d[e], j + e));
         });
       else
-        r.first_sweep(j0, j1, base, [&](int, const float (&d)[4]) {
+        r.first_sweep(j0, j1, [&](int, const float (&d)[4]) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float w = R::weight(d[e]);
@@ -858,8 +982,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   before = __shfl_sync(0xffffffffu, before, owner);
   const int j0 = part / kSubs * chunk + part % kSubs * r.sub;
   for (int j = j0 + 4 * lane;; j += kStep) {
-    const float4 f = r.quad(j);
-    const float d[4] = {f.x, f.y, f.z, f.w};
+    float d[4];
+    if constexpr (RESIDENT) {
+      const float4 f = r.quad(j);
+      d[0] = f.x;
+      d[1] = f.y;
+      d[2] = f.z;
+      d[3] = f.w;
+    } else {
+      r.dist4(r.load4(j), d);
+    }
     uint64_t q[4], sum4 = 0;
 #pragma unroll
     for (int e = 0; e < 4; ++e) sum4 += q[e] = mass_of(kept_weight(d[e], j + e));
@@ -895,13 +1027,21 @@ void launch_sample_tokens(const SampleArgs& a, cudaStream_t stream) {
   if (a.V < 1 || a.V > sample_max_vocabulary()) throw std::invalid_argument("sample_tokens: vocabulary size");
   int C = 1;
   while (slice_positions(a.V, C) > kSlice) C *= 2;
-  // Few rows: more CTAs for each while two fit every SM.
-  while (C < kMaxCluster && slice_positions(a.V, C) > 4096 && int64_t(a.R) * C * 2 <= 2 * sm_count()) C *= 2;
+  // Many rows that do not fit one CTA's shared memory: a CTA per row that reads it three times (the last two
+  // from L2) instead of a cluster that keeps it.  It needs no cluster barriers and less per-row bookkeeping,
+  // but one SM's time per row.  Measured on B200, top-p over 129,280 logits, streamed / resident: 148 rows
+  // 182 / 170 us, 200 rows 250 / 221, 256 rows 256 / 272; 512 rows of 50,000 logits 147 / 211.
+  const bool resident = C == 1 || a.R < sm_count() * 3 / 2;
+  if (!resident) C = 1;
+  // Few rows: more CTAs for each while two fit every SM (one row of 129,280: 31 us with 8, 25 us with 16).
+  while (resident && C < kMaxCluster && slice_positions(a.V, C) > 4096 && int64_t(a.R) * C * 2 <= 2 * sm_count()) C *= 2;
   const int chunk = (slice_positions(a.V, C) + kWarps * kStep - 1) / (kWarps * kStep) * kStep;
-  const size_t smem = sizeof(Shared) + size_t(chunk) * kWarps * 4;
-  auto kernel = a.bf16 ? sample_kernel<true> : sample_kernel<false>;
+  const size_t smem = sizeof(Shared) + (resident ? size_t(chunk) * kWarps * 4 : 0);
+  auto kernel = a.bf16 ? (resident ? sample_kernel<true, true> : sample_kernel<true, false>)
+                       : (resident ? sample_kernel<false, true> : sample_kernel<false, false>);
   once_per_device<Shared>([] {
-    for (auto* k : {sample_kernel<true>, sample_kernel<false>}) {
+    for (auto* k : {sample_kernel<true, true>, sample_kernel<false, true>, sample_kernel<true, false>,
+                    sample_kernel<false, false>}) {
       cuda_check(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(Shared) + kSlice * 4)),
                  "sample_tokens smem");
       cuda_check(cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "sample_tokens cluster");
