@@ -103,6 +103,7 @@ struct Small {
   int abort_flag;
 };
 constexpr size_t kSmemBytes = size_t(kOffSmall) + sizeof(Small);
+static_assert(MC * (DV * 2 + 16) <= kOffOwn - kOffQ && MC * (DV * 4 + 16) <= kOffP - kOffOwn, "staged output rows");
 static_assert(kSmemBytes <= 232448, "shared_prefix_mla: shared memory over the per-block limit");
 
 // Work list: units [0, full) are whole row tiles; units [full, full + cut) are
@@ -272,6 +273,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x / 32;
   const int lane = threadIdx.x % 32;
 
+  if (threadIdx.x == 32) {
+    tma_prefetch_desc(&tma_q);
+    tma_prefetch_desc(&tma_kv);
+  }
   if (threadIdx.x == 0) {
     mbar_init(&s.q_full, 2);
     for (int i = 0; i < STAGES; ++i) {
@@ -637,11 +642,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (have_o) tc_fence_after();
     const int trow = MC * int(crank) + hrow;  // row within the tile
     const int64_t row = w.row0 + trow;
-    // O leaves through shared memory (the operands are no longer needed), so that a warp writes whole rows:
-    // straight from the registers every store would touch 32 rows.  16-byte units are XORed with the row.
+    // O leaves through shared memory (the operands are no longer needed) and one bulk copy per row: straight
+    // from the registers every store would touch 32 rows.  Rows are 16 bytes further apart than they are
+    // long, so that eight neighbouring rows' 16-byte units lie in different banks.
     // Warpgroup wg holds value half wg: columns [128 wg, +128) = dims 256 wg + 128 kh + [0, 128).
     if (w.slot < 0 || have_o) {
+      const uint32_t row_bytes = w.slot < 0 ? DV * 2 : DV * 4;
       const uint32_t stage = sbase + (w.slot < 0 ? kOffQ : kOffOwn);
+      const uint32_t my_row = stage + hrow * (row_bytes + 16);
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         uint32_t r[32];
@@ -659,7 +667,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int j = 0; j < 32; j += 8)
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
-                             stage + hrow * (DV * 2) + ((((dim0 + j) >> 3) ^ (hrow & 7)) << 4)),
+                             my_row + (dim0 + j) * 2),
                          "r"(pack_bf16(scaled(j), scaled(j + 1))), "r"(pack_bf16(scaled(j + 2), scaled(j + 3))),
                          "r"(pack_bf16(scaled(j + 4), scaled(j + 5))), "r"(pack_bf16(scaled(j + 6), scaled(j + 7)))
                          : "memory");
@@ -667,26 +675,21 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int j = 0; j < 32; j += 4)
             asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(
-                             stage + hrow * (DV * 4) + ((((dim0 + j) >> 2) ^ (hrow & 7)) << 4)),
+                             my_row + (dim0 + j) * 4),
                          "f"(scaled(j)), "f"(scaled(j + 1)), "f"(scaled(j + 2)), "f"(scaled(j + 3))
                          : "memory");
         }
       }
+      fence_proxy_async();
       named_barrier(3, kSoftmaxThreads);
-      // One row of 16-byte units per warp and step: 64 units (BF16) or 128 (FP32 partials).
-      const int units = w.slot < 0 ? DV * 2 / 16 : DV * 4 / 16;
-      for (int rr = warp; rr < MC; rr += kSoftmaxWarps) {
-        const int tr = MC * int(crank) + rr;
-        if (w.slot < 0 && tr >= w.nrows) break;
-        uint8_t* dst = w.slot < 0 ? reinterpret_cast<uint8_t*>(a.out + (int64_t(w.row0) + tr) * DV)
-                                  : reinterpret_cast<uint8_t*>(part_o + (int64_t(w.slot) * BM + tr) * DV);
-        for (int u = lane; u < units; u += 32) {
-          uint4 q;
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w)
-                       : "r"(stage + rr * units * 16 + ((u ^ (rr & 7)) << 4)));
-          *reinterpret_cast<uint4*>(dst + u * 16) = q;
-        }
+      const int tr = MC * int(crank) + tt;
+      if (tt < MC && (w.slot >= 0 || tr < w.nrows)) {
+        const void* dst = w.slot < 0 ? static_cast<const void*>(a.out + (int64_t(w.row0) + tr) * DV)
+                                     : static_cast<const void*>(part_o + (int64_t(w.slot) * BM + tr) * DV);
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst),
+                     "r"(stage + tt * (row_bytes + 16)), "r"(row_bytes)
+                     : "memory");
+        asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
       }
     }
     if (wg == 0 && kh == 0) {
@@ -731,27 +734,44 @@ __global__ void __launch_bounds__(DV / 4) prefix_mla_merge_kernel(const __grid_c
     const int g = int(row / a.H), h = int(row % a.H);
     tail = (mp.tail_slot0 + int64_t(g) * ((a.H + BM - 1) / BM) + h / BM) * BM + h % BM;
   }
-  float mx = -INFINITY;
-  for (int s = s0; s < s1; ++s) mx = fmaxf(mx, part_lse[int64_t(s) * BM + lane]);
-  if (tail >= 0) mx = fmaxf(mx, part_lse[tail]);
+  // Weights exp(lse_s - max) of up to 128 partials at a time (a row tile has at most one per SM pair): one
+  // thread per partial, so that the partials' rows are then loaded without waiting for one another.
+  __shared__ float weight[DV / 4], red[2][4];
+  const int n = s1 - s0 + (tail >= 0 ? 1 : 0);
+  float lse = -INFINITY;
+  if (int(threadIdx.x) < n) {
+    const int s = s0 + int(threadIdx.x);
+    lse = part_lse[s < s1 ? int64_t(s) * BM + lane : tail];
+  }
+  float mx = lse;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  if (threadIdx.x % 32 == 0) red[0][threadIdx.x / 32] = mx;
+  __syncthreads();
+  mx = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
   const float base = mx == -INFINITY ? 0.f : mx;
+  // -inf: nothing visible there, the partial was not written.
+  const float wt = lse == -INFINITY ? 0.f : expf(lse - base);
+  weight[threadIdx.x] = wt;
+  float wsum = wt;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) wsum += __shfl_xor_sync(0xffffffffu, wsum, o);
+  if (threadIdx.x % 32 == 0) red[1][threadIdx.x / 32] = wsum;
+  __syncthreads();
+  wsum = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float wsum = 0.f;
-  auto add = [&](int64_t r) {
-    const float lse = part_lse[r];
-    // -inf: nothing visible there, the partial was not written.
-    const float wt = lse == -INFINITY ? 0.f : expf(lse - base);
-    const float4 p = lse == -INFINITY ? make_float4(0.f, 0.f, 0.f, 0.f)
-                                      : *reinterpret_cast<const float4*>(part_o + r * DV + d0);
-    wsum += wt;
-    acc.x = fmaf(wt, p.x, acc.x);
-    acc.y = fmaf(wt, p.y, acc.y);
-    acc.z = fmaf(wt, p.z, acc.z);
-    acc.w = fmaf(wt, p.w, acc.w);
+  auto add = [&](int k, int64_t r) {
+    const float wk = weight[k];
+    if (wk == 0.f) return;
+    const float4 p = *reinterpret_cast<const float4*>(part_o + r * DV + d0);
+    acc.x = fmaf(wk, p.x, acc.x);
+    acc.y = fmaf(wk, p.y, acc.y);
+    acc.z = fmaf(wk, p.z, acc.z);
+    acc.w = fmaf(wk, p.w, acc.w);
   };
-#pragma unroll 4
-  for (int s = s0; s < s1; ++s) add(int64_t(s) * BM + lane);
-  if (tail >= 0) add(tail);
+#pragma unroll 8
+  for (int s = s0; s < s1; ++s) add(s - s0, int64_t(s) * BM + lane);
+  if (tail >= 0) add(n - 1, tail);
   const float inv = wsum == 0.f ? 0.f : 1.f / wsum;
   *reinterpret_cast<uint2*>(a.out + row * DV + d0) =
       make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
