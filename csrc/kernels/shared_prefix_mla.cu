@@ -811,6 +811,9 @@ void make_plan(const PrefixMLAArgs& a, FullPlan& f) {
     // idle pairs would save exceeds the extra units' cost.
     const int64_t work = int64_t(rest) * p.tiles;
     shares = int(std::min<int64_t>(pairs, work / kMinShareTiles));
+    // The same cuts in every row tile, where that idles less than a tenth of the pairs: the tiles then walk the
+    // prefix side by side (each record leaves HBM once) and no share straddles two of them.
+    if (rest > 0 && shares % rest * 10 <= shares) shares -= shares % rest;
     if (shares <= rest || p.tiles * (1. - double(rest) / shares) * kTileUs < (p.apart ? 0. : kShareUs + kMergeUs)) {
       p.full = rt;
       rest = 0;
@@ -842,7 +845,7 @@ void make_plan(const PrefixMLAArgs& a, FullPlan& f) {
       }
     }
     m.begin[rest] = p.slots;
-    std::sort(p.share, p.share + p.cut, [](const Share& x, const Share& y) { return x.t1 - x.t0 > y.t1 - y.t0; });
+    std::stable_sort(p.share, p.share + p.cut, [](const Share& x, const Share& y) { return x.t1 - x.t0 > y.t1 - y.t0; });
   }
   if (p.apart && !only_tails) {
     m.tail_slot0 = p.slots;
