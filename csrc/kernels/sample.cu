@@ -9,7 +9,7 @@
 // The masses are whole numbers, so sums do not depend on their order: a draw
 // is the same whatever the batch, the split over threads or the kernel.
 //
-// The order is never sorted: a histogram of d (1,024 bins, counts and masses)
+// The order is never sorted: a histogram of d (1,024 or 2,048 bins, counts and masses)
 // finds the bins in which the filters cut, and the few entries of those bins
 // are ranked against each other.  When they do not fit the list (equal or
 // clustered logits), the bin is split again by the bits of the logits until it
@@ -35,7 +35,9 @@ constexpr int kMaxCluster = 16;
 constexpr int kStep = 128;               // positions per warp step (4 per lane)
 constexpr int kSubs = 4;                 // parts of a warp's positions whose kept masses are summed apart
 constexpr int kSlice = 16384;            // positions of a CTA, at most (16 of them padding at least)
-constexpr int kBins = 1024;
+// Bins of the histogram: of a resident row (two CTAs' slices and histograms fill an SM's shared memory) and of
+// a streamed one.
+constexpr int kBinsResident = 1024, kBinsStreamed = 2048;
 constexpr int kList = 512;
 constexpr float kFixed = 68719476736.f;  // 2^36
 constexpr float kSpan = 25.f;            // exp(-25) * 2^36 < 1: entries further down have no mass
@@ -43,8 +45,8 @@ constexpr float kTiny = 0x1p-60f;        // distances below it are told apart by
 constexpr uint64_t kNothing = ~0ull;     // composite above every entry
 constexpr uint64_t kInK = 1ull << 63, kInP = 1ull << 62;  // list entry belongs to the bin(s) of the top-k / top-p cut
 constexpr uint64_t kMassBits = kInP - 1;
-static_assert(kBins == 2 * kThreads, "two bins per thread");
 
+template <int kBins>
 struct alignas(16) Shared {
   uint64_t xch[2][2][kMaxCluster];  // exchanged values (double buffered)
   uint64_t decision[2];             // written by the CTA that owns an equal-value cut (double buffered)
@@ -130,7 +132,10 @@ __device__ __forceinline__ uint64_t warp_inclusive64(uint64_t v) {
 // every pass reads it again.
 template <bool BF16, bool RESIDENT>
 struct Row {
-  Shared& s;
+  static constexpr int kBins = RESIDENT ? kBinsResident : kBinsStreamed;
+  static constexpr int kPer = kBins / kThreads;  // bins of a thread: [kPer * thread, + kPer)
+  using Sh = Shared<kBins>;
+  Sh& s;
   float* v;                // logits, then d
   const void* src;
   int C, rank;
@@ -140,7 +145,7 @@ struct Row {
   bool usual;              // no scaling
   int phase = 0, turn = 0, event = 0, gathers = 0;  // buffers in use
 
-  __device__ Row(Shared& s_) : s(s_) {}
+  __device__ Row(Sh& s_) : s(s_) {}
 
   __device__ float logit(int i) const {
     if constexpr (BF16) return clean(__bfloat162float(static_cast<const __nv_bfloat16*>(src)[i]));
@@ -284,8 +289,8 @@ struct Row {
   __device__ void fold(bool first) {
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int b = 2 * threadIdx.x + i;
+    for (int i = 0; i < kPer; ++i) {
+      const int b = kPer * threadIdx.x + i;
       const uint64_t m = (uint64_t(s.hi[b]) << 18) + s.lo[b];
       s.all_cnt[b] = first ? s.cnt[b] : s.all_cnt[b] + s.cnt[b];
       s.all_mass[b] = first ? m : s.all_mass[b] + m;
@@ -307,15 +312,15 @@ struct Row {
     }
   }
   // CTA c sums the bins [c, c + 1) * kBins / C of all CTAs and hands them to all; every thread then holds
-  // what lies before its two bins.
+  // what lies before its own.
   __device__ void merge() {
     cluster_sync();
     if constexpr (!RESIDENT) {
       // folded already
     } else if (C == 1) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int b = 2 * threadIdx.x + i;
+      for (int i = 0; i < kPer; ++i) {
+        const int b = kPer * threadIdx.x + i;
         s.all_cnt[b] = s.cnt[b];
         s.all_mass[b] = (uint64_t(s.hi[b]) << 18) + s.lo[b];
       }
@@ -348,13 +353,18 @@ struct Row {
     }
     scan();
   }
-  uint32_t before_cnt;              // in the bins before the thread's two
+  uint32_t before_cnt;              // in the bins before the thread's
   uint64_t before_mass;
   uint64_t total_count, total_mass;
   __device__ void scan() {  // (the thread's own bins were written by itself when C == 1)
-    const int b = 2 * threadIdx.x, warp = threadIdx.x / 32;
-    const uint32_t c = s.all_cnt[b] + s.all_cnt[b + 1];
-    const uint64_t m = s.all_mass[b] + s.all_mass[b + 1];
+    const int warp = threadIdx.x / 32;
+    uint32_t c = 0;
+    uint64_t m = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      c += s.all_cnt[kPer * threadIdx.x + i];
+      m += s.all_mass[kPer * threadIdx.x + i];
+    }
     const uint64_t mi = warp_inclusive64(m);
     uint32_t ci = c;
 #pragma unroll
@@ -440,8 +450,8 @@ struct Row {
     __syncthreads();
     uint64_t c = count0 + before_cnt, m = mass0 + before_mass;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int b = 2 * threadIdx.x + i;
+    for (int i = 0; i < kPer; ++i) {
+      const int b = kPer * threadIdx.x + i;
       const uint64_t ce = c + s.all_cnt[b], me = m + s.all_mass[b];
       if (!g.reached(c, m) && g.reached(ce, me)) {
         s.found[0] = b;
@@ -659,8 +669,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   extern __shared__ __align__(16) uint8_t smem_raw[];
   pdl_trigger();
   pdl_wait();
-  Shared& s = *reinterpret_cast<Shared*>(smem_raw);
   using R = Row<BF16, RESIDENT>;
+  using Sh = typename R::Sh;
+  constexpr int kBins = R::kBins;
+  Sh& s = *reinterpret_cast<Sh*>(smem_raw);
   constexpr int VEC = BF16 ? 8 : 4;
   constexpr int kSize = BF16 ? 2 : 4;
   const int64_t row = blockIdx.x / C;
@@ -669,7 +681,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   r.C = C;
   r.rank = int(blockIdx.x % C);
   r.src = static_cast<const uint8_t*>(a.logits) + row * a.ld * kSize;
-  r.v = reinterpret_cast<float*>(smem_raw + sizeof(Shared));
+  r.v = reinterpret_cast<float*>(smem_raw + sizeof(Sh));
   const float T = a.temperature ? a.temperature[row] : a.temperature0;
   const int k = a.top_k ? a.top_k[row] : a.top_k0;
   const float p = a.top_p ? a.top_p[row] : a.top_p0;
@@ -1020,6 +1032,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
 // Positions of a CTA: whole vectors of 8, plus 8 of padding in the first.
 static int slice_positions(int V, int C) { return ((V + 7) / 8 + C - 1) / C * 8 + 16; }
 
+constexpr int kMaxSmem = int(sizeof(Shared<kBinsResident>) + kSlice * 4);
+static_assert(sizeof(Shared<kBinsStreamed>) <= kMaxSmem && 2 * (kMaxSmem + 1024) <= 233472, "two CTAs per SM");
+
 int sample_max_vocabulary() { return kMaxCluster * (kSlice - 32); }
 
 void launch_sample_tokens(const SampleArgs& a, cudaStream_t stream) {
@@ -1036,13 +1051,13 @@ void launch_sample_tokens(const SampleArgs& a, cudaStream_t stream) {
   // Few rows: more CTAs for each while two fit every SM (one row of 129,280: 31 us with 8, 25 us with 16).
   while (resident && C < kMaxCluster && slice_positions(a.V, C) > 4096 && int64_t(a.R) * C * 2 <= 2 * sm_count()) C *= 2;
   const int chunk = (slice_positions(a.V, C) + kWarps * kStep - 1) / (kWarps * kStep) * kStep;
-  const size_t smem = sizeof(Shared) + (resident ? size_t(chunk) * kWarps * 4 : 0);
+  const size_t smem = resident ? sizeof(Shared<kBinsResident>) + size_t(chunk) * kWarps * 4 : sizeof(Shared<kBinsStreamed>);
   auto kernel = a.bf16 ? (resident ? sample_kernel<true, true> : sample_kernel<true, false>)
                        : (resident ? sample_kernel<false, true> : sample_kernel<false, false>);
-  once_per_device<Shared>([] {
+  once_per_device<Shared<kBinsResident>>([] {
     for (auto* k : {sample_kernel<true, true>, sample_kernel<false, true>, sample_kernel<true, false>,
                     sample_kernel<false, false>}) {
-      cuda_check(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(Shared) + kSlice * 4)),
+      cuda_check(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem),
                  "sample_tokens smem");
       cuda_check(cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "sample_tokens cluster");
     }
