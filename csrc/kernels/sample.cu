@@ -19,6 +19,12 @@
 // stays in their shared memory for all later passes (first as logits, then as
 // d); with many long rows, one CTA per row reads it again instead.  The CTAs exchange values through distributed shared memory.  Nothing
 // spins: they meet at hardware barriers only (six per row with one filter, two without).
+//
+// Measured on B200: one row of 129,280 FP32 logits with top-k and top-p 19 us
+// (its bytes take 0.1 us: the barriers and exchanges between CTAs are the
+// bound), 16 rows 29 us; 256 rows with top-p 198 us, streamed, against 20 us
+// for their bytes: bound by instruction issue (94 warp instructions per 32
+// logits; a quotient, two exponentials and two histogram additions each).
 #include <algorithm>
 #include <cmath>
 

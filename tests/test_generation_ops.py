@@ -509,3 +509,95 @@ def test_launch_counts():
     n = launch_count()
     ops.sample_tokens(x, u)
     assert launch_count() - n == 1
+
+
+@gpu
+def test_shared_prefix_mla_offsets_past_32_bits():
+    """Prefix rows and tails that lie further apart than 2^31 elements."""
+    q, prefix, tail = prefix_inputs(2, 1, 128, 130, 40, "cuda", seed=8)
+    want = ops.shared_prefix_mla(q, prefix, tail, None, SCALE)
+    step = 2**24 + 8                                    # 130 rows: 2.2e9 elements
+    store = torch.empty(step * 130, dtype=torch.bfloat16, device="cuda")
+    far = store.as_strided((130, 576), (step, 1))
+    far.copy_(prefix)
+    far_tail = store.as_strided((2, 40, 576), (2**31 + 2**20, 2**16, 1), 600)  # between the prefix rows
+    far_tail.copy_(tail)
+    got = ops.shared_prefix_mla(q, far, far_tail, None, SCALE)
+    assert torch.equal(got, want)
+
+
+@gpu
+@pytest.mark.parametrize("B,T,H,P,S", [(2, 70, 128, 90, 70), (300, 1, 16, 40, 3), (3, 5, 130, 64, 9)])
+def test_shared_prefix_mla_many_queries(B, T, H, P, S):
+    """More query tokens than a row tile has rows; many small queries; a head count just over a tile."""
+    q, prefix, tail = prefix_inputs(B, T, H, P, S, "cuda", seed=9)
+    lens = torch.randint(0, S + 1, (B,), generator=torch.Generator().manual_seed(10))
+    out, lse = ops.shared_prefix_mla(q, prefix, tail, lens.int().cuda(), SCALE, return_lse=True)
+    keep = sorted({0, 1, B // 2, B - 1})
+    check_prefix(q[keep], prefix, tail[keep], lens[keep].tolist(), out[keep], lse[keep])
+
+
+@gpu
+def test_sample_offsets_past_32_bits():
+    x, u = rows(3, 5000, seed=11, dtype=torch.bfloat16)
+    want = ops.sample_tokens(x, u, top_k=50)
+    store = torch.empty(2 * (2**31 + 16) + 5000, dtype=torch.bfloat16, device="cuda")
+    far = store.as_strided((3, 5000), (2**31 + 16, 1))
+    far.copy_(x)
+    for a, b in zip(ops.sample_tokens(far, u, top_k=50), want):
+        assert torch.equal(a, b)
+
+
+@gpu
+@pytest.mark.parametrize("R", [16, 300])  # rows kept in shared memory, and rows read again
+def test_sample_per_row_values_that_numbers_may_not_have(R):
+    """Device values are not checked: the documented meaning of each odd one."""
+    inf, nan = math.inf, math.nan
+    V = 40001
+    x, u = rows(R, V, seed=12)
+    i = torch.arange(R, device="cuda")
+    best = x.argmax(-1)
+
+    def draw(**kw):
+        return ops.sample_tokens(x, u, **{k: torch.tensor(v, dtype=torch.int32 if k == "top_k" else torch.float32,
+                                                          device="cuda")[i % len(v)] for k, v in kw.items()})
+
+    tok, lp = draw(temperature=[nan, -1.0, 0.0, -inf])
+    assert torch.equal(tok, best) and not lp.any()
+    for kw in (dict(top_p=[-1.0, 0.0]), dict(min_p=[2.0, inf]), dict(top_k=[1]), dict(temperature=[1e-30, 1e-44])):
+        tok, _ = draw(**kw)
+        assert torch.equal(tok, best)
+    for a, b in zip(draw(top_k=[0, -5], top_p=[nan, 1.0, 7.0], min_p=[nan, -1.0, 0.0]), ops.sample_tokens(x, u)):
+        assert torch.equal(a, b)
+    tok, lp = draw(temperature=[1e30, inf])  # flat: the vocabulary in equal parts
+    at = u.double() * V
+    sure = (at - at.round()).abs() > 2.0**-15
+    assert torch.equal(tok[sure], at.floor().long()[sure])
+    assert (lp + math.log(V)).abs().max() < 1e-5
+
+
+@gpu
+@pytest.mark.parametrize("params", [dict(top_p=0.7), dict(top_k=3000), dict(top_k=20000, top_p=0.9),
+                                    dict(top_p=0.9, min_p=0.05), dict(top_k=500, top_p=0.6, min_p=0.01)], ids=str)
+@pytest.mark.parametrize("R", [7, 260])
+@pytest.mark.parametrize("kind", ["flat", "coarse", "two", "masked"])
+def test_sample_clustered_rows(params, R, kind):
+    """Rows whose cut falls among many nearly equal or equal logits: finer bins, then the keys' bits, then indices.
+    Such draws hang on the last bit of the weights, so the oracle runs on the GPU with the same exponential."""
+    V = 50021
+    x, u = rows(R, V, seed=13)
+    if kind == "flat":
+        x = x * 0.02
+    elif kind == "coarse":
+        x = (x * 2).round() / 2
+    elif kind == "two":
+        x = torch.where(x > 1.0, 1.0, 0.5)
+    else:
+        x[:, ::3] = -math.inf
+        x[:, 1::5] = math.nan
+    tok, lp = ops.sample_tokens(x, u, **params)
+    few = list(range(0, R, max(1, R // 6)))
+    want, want_lp = ref.sample_tokens(x[few], u[few], 1.0, params.get("top_k", 0), params.get("top_p", 1.0),
+                                      params.get("min_p", 0.0))
+    assert torch.equal(tok[few], want)
+    assert ((lp[few] - want_lp).abs() <= 2.0**-21 * (1 + want_lp.abs())).all()
