@@ -369,6 +369,31 @@ def bench_rs_gemm(M=1024, N=7168, Kdim=2304, **_):
             "tflops": flops / ms / 1e9}
 
 
+def bench_shared_prefix_mla(B=64, P=16384, S=64, H=128, **_):
+    """B continuations of one P-row history with S-row tails (one query token each)."""
+    dev = "cuda"
+    g = torch.Generator(device=dev).manual_seed(0)
+    q = (torch.randn(B, H, 576, device=dev, generator=g) * 0.5).bfloat16()
+    prefix = torch.randn(P, 576, device=dev, generator=g).bfloat16()
+    tail = torch.randn(B, S, 576, device=dev, generator=g).bfloat16()
+    ms = time_fn(lambda: ops.shared_prefix_mla(q, prefix, tail, None, 0.1352))
+    flops = 2.0 * B * H * (P + S) * (576 + 512)
+    return {"op": "shared_prefix_mla", "B": B, "P": P, "S": S, "H": H, "ms": ms, "tflops": flops / ms / 1e9,
+            **roofline(ms, flops=flops, nbytes=(P + B * S) * 1152 + B * H * (576 + 512) * 2)}
+
+
+def bench_sample(R=256, V=129280, temperature=0.8, top_k=0, top_p=0.9, **_):
+    """One draw per row of R x V FP32 logits (Gaussian bulk, exponential tail)."""
+    dev = "cuda"
+    g = torch.Generator(device=dev).manual_seed(0)
+    x = torch.randn(R, V, device=dev, generator=g) * 2
+    x -= torch.rand((R, V), device=dev, generator=g).clamp_min_(1e-12).log_() * 1.1
+    u = torch.rand(R, device=dev, generator=g)
+    ms = time_fn(lambda: ops.sample_tokens(x, u, temperature=temperature, top_k=top_k, top_p=top_p))
+    return {"op": "sample", "R": R, "V": V, "temperature": temperature, "top_k": top_k, "top_p": top_p, "ms": ms,
+            "read_gbs": R * V * 4 / ms / 1e6, **roofline(ms, nbytes=R * V * 4 + R * 16)}
+
+
 def bench_copy_curve(**_):
     """Device-to-device copy time against size (L2 flushed before each call): the
     size-dependent floor of any kernel that streams that many bytes once
@@ -390,7 +415,8 @@ def bench_copy_curve(**_):
 OPS = {"sparse_mla": bench_sparse_mla, "fp8_gemm": bench_fp8_gemm, "indexer": bench_indexer,
        "indexer_select": bench_indexer_select, "topk": bench_topk, "decode_gemms": bench_decode_gemms,
        "ag_gemm": bench_ag_gemm, "rs_gemm": bench_rs_gemm, "copy_curve": bench_copy_curve,
-       "gemm_paths": bench_gemm_paths, "gemv_ksplit": bench_gemv_ksplit}
+       "gemm_paths": bench_gemm_paths, "gemv_ksplit": bench_gemv_ksplit,
+       "shared_prefix_mla": bench_shared_prefix_mla, "sample": bench_sample}
 
 
 def main():
@@ -406,6 +432,11 @@ def main():
     p.add_argument("--clustered", action="store_true")
     p.add_argument("--order", default="value", choices=("value", "index"), help="topk: output order")
     p.add_argument("--causal", action="store_true", help="topk: rows end at N - R + r (prefill chunk)")
+    p.add_argument("--B", type=int, default=64, help="shared_prefix_mla: continuations")
+    p.add_argument("--prefix", type=int, default=16384, help="shared_prefix_mla: history rows")
+    p.add_argument("--rows", type=int, default=256, help="sample: rows of logits")
+    p.add_argument("--top-k", type=int, default=0, help="sample")
+    p.add_argument("--top-p", type=float, default=0.9, help="sample")
     p.add_argument("--M", type=int, default=1024)
     p.add_argument("--N", type=int, default=36864)
     p.add_argument("--Kdim", type=int, default=7168)
@@ -427,6 +458,10 @@ def main():
             kw = dict(Q=a.R)
         if name in ("decode_gemms", "gemm_paths"):
             kw = dict(M=a.M)
+        if name == "shared_prefix_mla":
+            kw = dict(B=a.B, P=a.prefix)
+        if name == "sample":
+            kw = dict(R=a.rows, top_k=a.top_k, top_p=a.top_p)
         if name == "topk":
             kw = dict(R=a.R, clustered=a.clustered, order=a.order, causal=a.causal)
         print(json.dumps(OPS[name](**kw)))
