@@ -439,6 +439,8 @@ std::tuple<Tensor, c10::optional<Tensor>> shared_prefix_mla(const Tensor& q, con
                   (!tail || tail->size(1) < (int64_t(1) << 30)),
               "more rows than 32-bit indices hold");
   c10::cuda::CUDAGuard g(q.device());
+  // A tensor map's rows do not overlap: broadcast or sliding prefixes are laid out first.
+  const Tensor rows = prefix.size(0) > 1 && prefix.stride(0) < 576 ? prefix.contiguous() : prefix;
   const Tensor qc = q.contiguous();
   if (reinterpret_cast<uintptr_t>(qc.data_ptr()) % 16) throw std::invalid_argument("q must start on a 16-byte boundary");
   auto shape = q.sizes().vec();
@@ -449,9 +451,9 @@ std::tuple<Tensor, c10::optional<Tensor>> shared_prefix_mla(const Tensor& q, con
   if (want_lse) lse = torch::empty(shape, q.options().dtype(torch::kFloat32));
   const Tensor lens = tail_lens ? tail_lens->contiguous() : Tensor();
   b200::PrefixMLAArgs a{};
-  a.q = cptr<__nv_bfloat16>(qc); a.prefix = cptr<__nv_bfloat16>(prefix); a.out = ptr<__nv_bfloat16>(out);
+  a.q = cptr<__nv_bfloat16>(qc); a.prefix = cptr<__nv_bfloat16>(rows); a.out = ptr<__nv_bfloat16>(out);
   a.B = B; a.T = T; a.H = H; a.P = prefix.size(0); a.scale = float(scale);
-  a.ld_prefix = prefix.size(0) > 1 ? prefix.stride(0) : 576;
+  a.ld_prefix = rows.size(0) > 1 ? rows.stride(0) : 576;
   a.err = err_ptr(q);
   if (tail) {
     a.tail = cptr<__nv_bfloat16>(*tail);

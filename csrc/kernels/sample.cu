@@ -9,16 +9,18 @@
 // The masses are whole numbers, so sums do not depend on their order: a draw
 // is the same whatever the batch, the split over threads or the kernel.
 //
-// The order is never sorted: a histogram of d (1,024 or 2,048 bins, counts and masses)
-// finds the bins in which the filters cut, and the few entries of those bins
-// are ranked against each other.  When they do not fit the list (equal or
-// clustered logits), the bin is split again by the bits of the logits until it
-// fits or holds one value, which is cut by index.
+// The order is never sorted: a histogram of d (1,024 or 2,048 bins, counts and
+// masses) finds the bins in which the filters cut, and the few entries of those
+// bins are ranked against each other.  When they do not fit the list (equal or
+// clustered logits), the bin is split into as many finer ones, and if that is
+// not enough by the bits of the logits until one value is left, which is cut by
+// index.
 //
 // A row belongs to a cluster of 1 to 16 CTAs: it is read from HBM once and
 // stays in their shared memory for all later passes (first as logits, then as
-// d); with many long rows, one CTA per row reads it again instead.  The CTAs exchange values through distributed shared memory.  Nothing
-// spins: they meet at hardware barriers only (six per row with one filter, two without).
+// d); with many long rows, one CTA per row reads it again instead.  The CTAs
+// exchange values through distributed shared memory.  Nothing spins: they meet
+// at hardware barriers only (six per row with one filter, two without).
 //
 // Measured on B200: one row of 129,280 FP32 logits with top-k and top-p 19 us
 // (its bytes take 0.1 us: the barriers and exchanges between CTAs are the
@@ -862,7 +864,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       __syncthreads();
       summed = true;
     };
-    // One cut in a bin with many entries: 1,024 finer bins of it, then the list, or the keys' bits if even a
+    // One cut in a bin with many entries: kBins finer bins of it, then the list, or the keys' bits if even a
     // finer bin does not fit (equal logits).
     auto settle = [&](const typename R::Cut& c, const typename R::Goal& g, bool by_k) {
       const float offset = 0.5f - float(c.bin);

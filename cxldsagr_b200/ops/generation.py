@@ -32,7 +32,8 @@ def shared_prefix_mla(q, prefix, tail, tail_lens, scale, *, return_lse: bool = F
     sees no record gives zeros.  With ``return_lse`` also the FP32 natural-log
     sum of exponentials [..., H] (-inf where nothing is visible), to merge with
     other parts of the attention.  On CUDA a length outside [0, S] is recorded
-    in the device error word (``check_errors``) and clamped.
+    in the device error word (``check_errors``) and clamped; with S = 0 the
+    lengths are not read.
     """
     B, D = q.shape[0], q.shape[-1]
     if q.dim() != 3 and q.dim() != 4:
@@ -81,7 +82,8 @@ def sample_tokens(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
 
     Returns (tokens int64 [R], log-probabilities FP32 [R] of the drawn tokens
     under the filtered distribution; 0 for temperature 0).  A row whose logits
-    are all -inf or NaN gives token -1 with log-probability -inf.
+    are all -inf or NaN gives token -1 with log-probability -inf.  On CUDA V is
+    at most 261,120.
     """
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError("logits must be [R, V] with V >= 1")

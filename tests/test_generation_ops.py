@@ -166,6 +166,16 @@ def test_shared_prefix_mla_views_and_streams():
 
 
 @gpu
+def test_shared_prefix_mla_broadcast_and_overlapping_records():
+    """One record or one tail for all (stride 0), and records that overlap in memory."""
+    q, one, tail = prefix_inputs(2, 1, 128, 70 * 8 + 576, 40, "cuda", seed=13)
+    for prefix in (one[:1].expand(70, 576), one.reshape(-1).as_strided((70, 576), (8, 1))):
+        for t in (tail, tail[:1].expand(2, 40, 576), tail[:, :1].expand(2, 40, 576)):
+            got = ops.shared_prefix_mla(q, prefix, t, None, SCALE)
+            assert torch.equal(got, ops.shared_prefix_mla(q, prefix.contiguous(), t.contiguous(), None, SCALE))
+
+
+@gpu
 def test_shared_prefix_mla_graph_follows_the_lengths():
     """Captured once, replayed while the tails grow (the lengths are read on the device)."""
     q, prefix, tail = prefix_inputs(4, 1, 128, 500, 130, "cuda", seed=5)
