@@ -47,10 +47,11 @@
 //
 // Measured on B200: 64 x 128 rows over 16,384 + 64 keys 225 us alone (1.30
 // PFLOP/s; 269 us back to back under the power limit), 4 x 128 rows over 65,536
-// keys 80 us with a cold L2, 2 x 128 rows over 64 keys 9 us.  A tile takes
+// keys 78 us with a cold L2, 2 x 128 rows over 64 keys 8 us.  A tile takes
 // 1,520 cycles per pair; the bound is the shared-memory reads of QK's operands
 // (N = 64 re-reads Q for every 64 keys: ~860 cycles a tile, PV ~600), next to
-// it the L2-to-SM path.  A record stage is held ~6,200 cycles from its load to
+// it the L2-to-SM path.  QK of two tiles at once (N = 128) reads Q half as often,
+// but has to wait for both tiles' records, and is slower: 260 against 229 us.  A record stage is held ~6,200 cycles from its load to
 // its PV, so four stages are needed to keep that pace: they fit because half of
 // P lies in the stage's RoPE chunk.  With three stages a tile took 2,080 cycles.
 #include <algorithm>
@@ -78,11 +79,9 @@ constexpr int kKeyChunkBytes = BNC * 128;
 constexpr int kPBytes = MC * 64;          // half of P: 64 rows x 32 keys BF16
 constexpr int kSoftmaxWarps = 8;          // warps 0-7
 constexpr int kSoftmaxThreads = kSoftmaxWarps * 32;
-constexpr int kOwnWarp0 = 8;              // warp 8: Q + records
-constexpr int kOwnWarps = 1;
+constexpr int kOwnWarp = 8;              // warp 8: Q + records
 constexpr int kPvMmaWarp = 9;             // CTA 0: issues PV
-constexpr int kPvWarp0 = 10;              // warp 10: peer keys' value dims
-constexpr int kPvWarps = 1;
+constexpr int kPvWarp = 10;              // warp 10: peer keys' value dims
 constexpr int kMmaWarp = 11;              // allocates TMEM; CTA 0: issues QK
 constexpr int kThreads = 12 * 32;
 constexpr uint32_t kQBytes = kChunks * kQChunkBytes;
@@ -202,11 +201,12 @@ __device__ __forceinline__ void mbar_arrive_expect_tx_at(uint32_t cluster_bar, u
   asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;" ::"r"(cluster_bar), "r"(bytes) : "memory");
 }
 
-// What a unit works on, the same in both CTAs and every role.
+// What a unit works on, the same in both CTAs and every role; seen and nt after see_tail.
 struct Unit {
   int row0, nrows;     // first flattened row, valid rows of the 128
   int p0, np;          // prefix tiles [p0, p0 + np)
-  int t0, nt;          // then tail tiles [t0, t0 + nt) of continuation b
+  int t0, nt;          // then tail tiles [t0, t0 + nt) of continuation b, at most up to t1
+  int t1, g;           // of query token g (-1: no tail)
   int b, seen;         // visible tail rows
   int64_t part;        // first of the unit's rows in the partials, -1: written directly
   __device__ int ntiles() const { return np + nt; }
@@ -228,7 +228,8 @@ __device__ __forceinline__ int visible_tail(const PrefixMLAArgs& a, int g) {
 __device__ __forceinline__ Unit decode_unit(const PrefixMLAArgs& a, const Plan& plan, int u) {
   Unit w;
   w.b = 0;
-  w.seen = w.t0 = w.nt = w.p0 = w.np = 0;
+  w.g = -1;
+  w.seen = w.t0 = w.t1 = w.nt = w.p0 = w.np = 0;
   const int rows = a.B * a.T * a.H;
   const int prefix_tiles = (a.P + BN - 1) / BN;
   if (u >= plan.full + plan.cut) {  // a query's tail
@@ -237,9 +238,9 @@ __device__ __forceinline__ Unit decode_unit(const PrefixMLAArgs& a, const Plan& 
     const int g = i / per, h0 = (i % per) * BM;
     w.row0 = g * a.H + h0;
     w.nrows = min(BM, a.H - h0);
+    w.g = g;
     w.b = g / a.T;
-    w.seen = visible_tail(a, g);
-    w.nt = (w.seen + BN - 1) / BN;
+    w.t1 = INT32_MAX;
     w.part = a.P > 0 ? int64_t(plan.slots) * BM + w.row0 : -1;  // one partial row per query row, after the slots
     return w;
   }
@@ -258,13 +259,18 @@ __device__ __forceinline__ Unit decode_unit(const PrefixMLAArgs& a, const Plan& 
   w.p0 = min(k0, prefix_tiles);
   w.np = min(k1, prefix_tiles) - w.p0;
   if (!plan.apart && k1 > prefix_tiles) {
-    const int g = w.row0 / a.H;
-    w.b = g / a.T;
-    w.seen = visible_tail(a, g);
+    w.g = w.row0 / a.H;
+    w.b = w.g / a.T;
     w.t0 = max(k0, prefix_tiles) - prefix_tiles;
-    w.nt = max(0, min(k1 - prefix_tiles, (w.seen + BN - 1) / BN) - w.t0);
+    w.t1 = k1 - prefix_tiles;
   }
   return w;
+}
+// The part that waits for a length from memory.
+__device__ __forceinline__ void see_tail(const PrefixMLAArgs& a, Unit& w) {
+  if (w.g < 0) return;
+  w.seen = visible_tail(a, w.g);
+  w.nt = max(0, min(w.t1, (w.seen + BN - 1) / BN) - w.t0);
 }
 
 __global__ void __launch_bounds__(kThreads, 1)
@@ -291,8 +297,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     mbar_init(&s.q_full, 2);
     for (int i = 0; i < STAGES; ++i) {
-      mbar_init(&s.own_full[i], 2 * kOwnWarps);
-      mbar_init(&s.pv_full[i], 2 * kPvWarps);
+      mbar_init(&s.own_full[i], 2);
+      mbar_init(&s.pv_full[i], 2);
       mbar_init(&s.pv_done[i], 1);
     }
     for (int i = 0; i < SBUF; ++i) {
@@ -316,8 +322,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_wait();
   pdl_trigger();
   tc_fence_after();
-  const Unit w = decode_unit(a, plan, int(blockIdx.x >> 1));
-  const int ntiles = w.ntiles();
+  Unit w = decode_unit(a, plan, int(blockIdx.x >> 1));
   auto own_chunk = [&](int st, int j) { return sbase + kOffOwn + (st * kChunks + j) * kKeyChunkBytes; };
   // PV's B operand (value dims, MN-major) of key half kh and value half v.
   auto pv_region = [&](int st, int kh, int v) { return own_chunk(st, 4 * v + 2 * kh); };
@@ -337,6 +342,28 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (crank == 0) mbar_arrive(bar);
     else mbar_arrive_remote(mapa_shared(smem_u32(bar), 0));
   };
+  // Prefix tile i's records and the Q rows of this CTA (one thread).
+  auto load_records = [&](int i) {
+    uint64_t* bar = &s.own_full[i % STAGES];
+    mbar_arrive_expect_tx_at(leader(bar), kOwnBytes);
+#pragma unroll 1
+    for (int j = 0; j < kChunks; ++j)
+      tma_load_pair(own_chunk(i % STAGES, j), &tma_kv, leader(bar), 64 * j, tile_key0(i) + BNC * int(crank));
+  };
+  auto load_q = [&]() {
+    mbar_arrive_expect_tx_at(leader(&s.q_full), kQBytes);
+#pragma unroll 1
+    for (int j = 0; j < kChunks; ++j)
+      tma_load_pair(sbase + kOffQ + j * kQChunkBytes, &tma_q, leader(&s.q_full), 64 * j, w.row0 + MC * int(crank));
+  };
+  // Q and the first prefix tiles do not wait for the tail's length.
+  const int ahead = min(w.np, STAGES);
+  if (warp == kOwnWarp && lane == 0 && ahead > 0) {
+    load_q();
+    for (int i = 0; i < ahead; ++i) load_records(i);
+  }
+  see_tail(a, w);
+  const int ntiles = w.ntiles();
   const uint8_t* tail_rows = reinterpret_cast<const uint8_t*>(a.tail + int64_t(w.b) * a.ld_batch);
   const int64_t tail_pitch = a.ld_tail * 2;
   // Rows [rows, 32) of key half kh's value dims in this CTA (one warp; 32 units of 16 bytes per row).
@@ -349,33 +376,19 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (ntiles == 0) {
     // nothing visible: straight to the epilogue
-  } else if (warp >= kOwnWarp0 && warp < kOwnWarp0 + kOwnWarps) {
+  } else if (warp == kOwnWarp) {
     // --------------------------------------------- Q rows + QK records
-    const int ow = warp - kOwnWarp0;
-    if (ow == 0 && lane == 0) {
-      mbar_arrive_expect_tx_at(leader(&s.q_full), kQBytes);
-#pragma unroll 1
-      for (int j = 0; j < kChunks; ++j)
-        tma_load_pair(sbase + kOffQ + j * kQChunkBytes, &tma_q, leader(&s.q_full), 64 * j, w.row0 + MC * int(crank));
-    }
-    for (int i = 0; i < ntiles; ++i) {
+    __syncwarp();
+    if (ahead == 0 && lane == 0) load_q();
+    for (int i = ahead; i < ntiles; ++i) {
       const int st = i % STAGES;
       if (!__all_sync(0xffffffffu, mbar_wait(&s.pv_done[st], ((i / STAGES) & 1) ^ 1, err, kErrTimeoutSmemEmpty,
                                              abort_flag)))
         break;
-      const int key0 = tile_key0(i) + BNC * int(crank);
       if (i < w.np) {
-        if (lane == 0) {
-          if (ow == 0) {
-            mbar_arrive_expect_tx_at(leader(&s.own_full[st]), kOwnBytes);
-#pragma unroll 1
-            for (int j = 0; j < kChunks; ++j)
-              tma_load_pair(own_chunk(st, j), &tma_kv, leader(&s.own_full[st]), 64 * j, key0);
-          } else {
-            arrive_leader(&s.own_full[st]);
-          }
-        }
+        if (lane == 0) load_records(i);
       } else {
+        const int key0 = tile_key0(i) + BNC * int(crank);
         // Visible rows by cp.async; of the others only the value dims have to be finite (their scores are
         // masked, but 0 * NaN would spread in PV): zeros.
         const int rows = min(max(w.seen - key0, 0), BNC);
@@ -397,9 +410,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       __syncwarp();
     }
-  } else if (warp >= kPvWarp0 && warp < kPvWarp0 + kPvWarps) {
+  } else if (warp == kPvWarp) {
     // ------------------------------------------- peer keys' value dims
-    const int pw = warp - kPvWarp0;
     const int peer = 1 - int(crank);
     for (int i = 0; i < ntiles; ++i) {
       const int st = i % STAGES;
@@ -410,15 +422,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int key0 = tile_key0(i) + BNC * peer;
       if (i < w.np) {
         if (lane == 0) {
-          if (pw == 0) {
-            mbar_arrive_expect_tx_at(leader(&s.pv_full[st]), kPvBytes);
+          mbar_arrive_expect_tx_at(leader(&s.pv_full[st]), kPvBytes);
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-              tma_load_pair(pv_region(st, peer, c >> 1) + (c & 1) * kKeyChunkBytes, &tma_kv, leader(&s.pv_full[st]),
-                            64 * (4 * (c >> 1) + 2 * int(crank) + (c & 1)), key0);
-          } else {
-            arrive_leader(&s.pv_full[st]);
-          }
+          for (int c = 0; c < 4; ++c)
+            tma_load_pair(pv_region(st, peer, c >> 1) + (c & 1) * kKeyChunkBytes, &tma_kv, leader(&s.pv_full[st]),
+                          64 * (4 * (c >> 1) + 2 * int(crank) + (c & 1)), key0);
         }
       } else {
         const int rows = min(max(w.seen - key0, 0), BNC);
@@ -653,9 +661,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (have_o) tc_fence_after();
     const int trow = MC * int(crank) + hrow;  // row within the tile
     const int64_t row = w.row0 + trow;
-    // O leaves through shared memory (the operands are no longer needed) and one bulk copy per row: straight
-    // from the registers every store would touch 32 rows.  Rows are 16 bytes further apart than they are
-    // long, so that eight neighbouring rows' 16-byte units lie in different banks.
+    // O leaves through shared memory (the operands are no longer needed) and a bulk copy per thread, of the 128
+    // dims that it wrote itself: straight from the registers every store would touch 32 rows.  Rows are 16 bytes
+    // further apart than they are long, so that eight neighbouring rows' 16-byte units lie in different banks.
     // Warpgroup wg holds value half wg: columns [128 wg, +128) = dims 256 wg + 128 kh + [0, 128).
     if (w.part < 0 || have_o) {
       const uint32_t row_bytes = w.part < 0 ? DV * 2 : DV * 4;
@@ -691,17 +699,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                          : "memory");
         }
       }
-      fence_proxy_async();
-      named_barrier(3, kSoftmaxThreads);
-      const int tr = MC * int(crank) + tt;
-      if (tt < MC && tr < w.nrows) {
-        const void* dst = w.part < 0 ? static_cast<const void*>(a.out + (int64_t(w.row0) + tr) * DV)
-                                     : static_cast<const void*>(part_o + (w.part + tr) * DV);
+      if (trow < w.nrows) {
+        const int dim0 = 256 * wg + 128 * kh;
+        const void* dst = w.part < 0 ? static_cast<const void*>(a.out + row * DV + dim0)
+                                     : static_cast<const void*>(part_o + (w.part + trow) * DV + dim0);
+        fence_proxy_async();
         asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst),
-                     "r"(stage + tt * (row_bytes + 16)), "r"(row_bytes)
+                     "r"(my_row + dim0 * (row_bytes / DV)), "r"(row_bytes / 4)
                      : "memory");
-        asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
       }
+      asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
     }
     if (wg == 0 && kh == 0) {
       if (trow >= w.nrows) {
@@ -747,14 +754,20 @@ __global__ void __launch_bounds__(DV / 4) prefix_mla_merge_kernel(const __grid_c
   }
   const int64_t tail = mp.tail_row0 >= 0 ? mp.tail_row0 + row : -1;
   // Weights exp(lse_s - max) of up to 128 partials at a time (a row tile has at most one per SM pair): one
-  // thread per partial, so that the partials' rows are then loaded without waiting for one another.
+  // thread per partial, so that the partials' rows are then loaded without waiting for one another.  The first
+  // eight are on their way before the weights are known, and dropped where nothing was written (24 x 16 heads
+  // over 4,096 rows 19.8 -> 17.4 us; 16 of them in registers: 0.5 us slower at 8 x 2,032 rows).
   __shared__ float weight[DV / 4], red[2][4];
   const int n = s1 - s0 + (tail >= 0 ? 1 : 0);
+  auto partial = [&](int k) { return k < s1 - s0 ? int64_t(s0 + k) * BM + lane : tail; };
   float lse = -INFINITY;
-  if (int(threadIdx.x) < n) {
-    const int s = s0 + int(threadIdx.x);
-    lse = part_lse[s < s1 ? int64_t(s) * BM + lane : tail];
-  }
+  if (int(threadIdx.x) < n) lse = part_lse[partial(int(threadIdx.x))];
+  auto load = [&](int k) { return *reinterpret_cast<const float4*>(part_o + partial(k) * DV + d0); };
+  constexpr int kFirst = 8;
+  float4 first[kFirst];
+#pragma unroll
+  for (int k = 0; k < kFirst; ++k)
+    if (k < n) first[k] = load(k);
   float mx = lse;
 #pragma unroll
   for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -772,18 +785,19 @@ __global__ void __launch_bounds__(DV / 4) prefix_mla_merge_kernel(const __grid_c
   __syncthreads();
   wsum = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto add = [&](int k, int64_t r) {
+  auto add = [&](int k, const float4& p) {
     const float wk = weight[k];
     if (wk == 0.f) return;
-    const float4 p = *reinterpret_cast<const float4*>(part_o + r * DV + d0);
     acc.x = fmaf(wk, p.x, acc.x);
     acc.y = fmaf(wk, p.y, acc.y);
     acc.z = fmaf(wk, p.z, acc.z);
     acc.w = fmaf(wk, p.w, acc.w);
   };
+#pragma unroll
+  for (int k = 0; k < kFirst; ++k)
+    if (k < n) add(k, first[k]);
 #pragma unroll 8
-  for (int s = s0; s < s1; ++s) add(s - s0, int64_t(s) * BM + lane);
-  if (tail >= 0) add(n - 1, tail);
+  for (int k = kFirst; k < n; ++k) add(k, load(k));
   const float inv = wsum == 0.f ? 0.f : 1.f / wsum;
   *reinterpret_cast<uint2*>(a.out + row * DV + d0) =
       make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
@@ -792,8 +806,10 @@ __global__ void __launch_bounds__(DV / 4) prefix_mla_merge_kernel(const __grid_c
 
 // How the row tiles are cut into shares.  Times in microseconds, measured on
 // B200: a 64-key tile, a share's start and end (launch, Q, filling the
-// pipeline, writing a partial), the merge kernel.
-constexpr double kTileUs = 0.8, kShareUs = 8., kMergeUs = 6.;
+// pipeline, writing a partial), the merge kernel, a wave of tails that finds no
+// free pairs (2 x 16 heads over 19,191 rows: 26 us with such a wave, 20 us with
+// two pairs left to the tails).
+constexpr double kTileUs = 0.8, kShareUs = 8., kMergeUs = 6., kTailWaveUs = 6.;
 constexpr int kMinShareTiles = 4;
 
 struct FullPlan {
@@ -823,10 +839,20 @@ void make_plan(const PrefixMLAArgs& a, FullPlan& f) {
     // Equal shares of the rest, one per pair (not shorter than kMinShareTiles), when what the
     // idle pairs would save exceeds the extra units' cost.
     const int64_t work = int64_t(rest) * p.tiles;
-    shares = int(std::min<int64_t>(pairs, work / kMinShareTiles));
+    // Tails that are apart take pairs of the same wave, where that costs the shares less than a wave of their own.
+    int room = pairs;
+    if (p.tails < pairs && work * kTileUs * p.tails < kTailWaveUs * pairs * (pairs - p.tails)) room = pairs - p.tails;
+    shares = int(std::min<int64_t>(room, work / kMinShareTiles));
     // The same cuts in every row tile, where that idles less than a tenth of the pairs: the tiles then walk the
-    // prefix side by side (each record leaves HBM once) and no share straddles two of them.
-    if (rest > 0 && shares % rest * 10 <= shares) shares -= shares % rest;
+    // prefix side by side (each record leaves HBM once) and no share straddles two of them.  Of the cuts with the
+    // same longest share those with the fewest partials.
+    if (rest > 0) {
+      const int most = std::min(room / rest, (p.tiles + kMinShareTiles - 1) / kMinShareTiles);
+      if (most > 0 && most * rest * 10 >= shares * 9) {
+        const int longest = (p.tiles + most - 1) / most;
+        shares = rest * ((p.tiles + longest - 1) / longest);
+      }
+    }
     if (shares <= rest || p.tiles * (1. - double(rest) / shares) * kTileUs < (p.apart ? 0. : kShareUs + kMergeUs)) {
       p.full = rt;
       rest = 0;
