@@ -28,6 +28,7 @@
 // for their bytes: bound by instruction issue (94 warp instructions per 32
 // logits; a quotient, two exponentials and two histogram additions each).
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "../common/host.h"
@@ -1045,23 +1046,43 @@ static_assert(sizeof(Shared<kBinsStreamed>) <= kMaxSmem && 2 * (kMaxSmem + 1024)
 
 int sample_max_vocabulary() { return kMaxCluster * (kSlice - 32); }
 
+// Launch configuration of `clusters` clusters of C CTAs (`attr` keeps the attributes).
+static cudaLaunchConfig_t cluster_config(int64_t clusters, int C, size_t smem, cudaLaunchAttribute (&attr)[2]) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(clusters * C), 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = C;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // the kernel starts with pdl_wait()
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cfg;
+}
+
+// Clusters of C CTAs (two CTAs per SM) that the device runs at a time.  A cluster stays within one group of
+// SMs, so these are fewer than the SMs would hold: 148, 71, 33 and 14 clusters of 2, 4, 8 and 16.
+static int clusters_at_a_time(int C) {
+  static std::atomic<int> cached[64][kMaxCluster + 1];
+  int device = 0;
+  cuda_check(cudaGetDevice(&device), "cudaGetDevice");
+  std::atomic<int>& known = cached[device & 63][C];
+  int n = known.load(std::memory_order_relaxed);
+  if (n == 0) {
+    cudaLaunchAttribute attr[2];
+    const cudaLaunchConfig_t cfg = cluster_config(1, C, kMaxSmem, attr);
+    cuda_check(cudaOccupancyMaxActiveClusters(&n, sample_kernel<false, true>, &cfg), "sample_tokens clusters");
+    known.store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
 void launch_sample_tokens(const SampleArgs& a, cudaStream_t stream) {
   if (a.R == 0) return;
   if (a.V < 1 || a.V > sample_max_vocabulary()) throw std::invalid_argument("sample_tokens: vocabulary size");
-  int C = 1;
-  while (slice_positions(a.V, C) > kSlice) C *= 2;
-  // Many rows that do not fit one CTA's shared memory: a CTA per row that reads it three times (the last two
-  // from L2) instead of a cluster that keeps it.  It needs no cluster barriers and less per-row bookkeeping,
-  // but one SM's time per row.  Measured on B200, top-p over 129,280 logits, streamed / resident: 148 rows
-  // 182 / 170 us, 200 rows 250 / 221, 256 rows 256 / 272; 512 rows of 50,000 logits 147 / 211.
-  const bool resident = C == 1 || a.R < sm_count() * 3 / 2;
-  if (!resident) C = 1;
-  // Few rows: more CTAs for each while two fit every SM (one row of 129,280: 31 us with 8, 25 us with 16).
-  while (resident && C < kMaxCluster && slice_positions(a.V, C) > 4096 && int64_t(a.R) * C * 2 <= 2 * sm_count()) C *= 2;
-  const int chunk = (slice_positions(a.V, C) + kWarps * kStep - 1) / (kWarps * kStep) * kStep;
-  const size_t smem = resident ? sizeof(Shared<kBinsResident>) + size_t(chunk) * kWarps * 4 : sizeof(Shared<kBinsStreamed>);
-  auto kernel = a.bf16 ? (resident ? sample_kernel<true, true> : sample_kernel<true, false>)
-                       : (resident ? sample_kernel<false, true> : sample_kernel<false, false>);
   once_per_device<Shared<kBinsResident>>([] {
     for (auto* k : {sample_kernel<true, true>, sample_kernel<false, true>, sample_kernel<true, false>,
                     sample_kernel<false, false>}) {
@@ -1070,19 +1091,34 @@ void launch_sample_tokens(const SampleArgs& a, cudaStream_t stream) {
       cuda_check(cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "sample_tokens cluster");
     }
   });
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(a.R) * C, 1, 1);
-  cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
+  int C = 1;
+  while (slice_positions(a.V, C) > kSlice) C *= 2;
+  // Many rows that do not fit one CTA's shared memory: a CTA per row that reads it three times (the last two
+  // from L2) instead of a cluster that keeps it.  It needs no cluster barriers and less per-row bookkeeping,
+  // but one SM's time per row.  Measured on B200, top-p over 129,280 logits, streamed / resident: 148 rows
+  // 182 / 170 us, 200 rows 250 / 221, 256 rows 256 / 272; 512 rows of 50,000 logits 147 / 211.
+  const bool resident = C == 1 || a.R < sm_count() * 3 / 2;
+  if (!resident) C = 1;
+  // More CTAs for each row while all clusters run at a time (16 rows of 129,280 logits take two turns with 16
+  // CTAs: 41 us, with 8: 29 us).  An exchange between CTAs costs about what 8,000 positions do, so one CTA keeps
+  // up to kAlone positions (5,000 logits with 1 / 2 / 4 CTAs 12.7 / 15.0 / 14.4 us, 9,000 14.2 / 16.0 / 15.6 us),
+  // of many rows all that fit it (60 rows of 13,000 16.8 / 20.8 us).  Of longer rows slices above kLong are cut
+  // (60 rows of 30,000 with 2 / 4 CTAs 26.3 / 23.1 us; but 24 rows of 18,673 18.1 / 20.1 us), with few rows
+  // shorter ones too (one row of 60,000 with 4 / 8 / 16 CTAs 20.7 / 18.1 / 17.5 us; 8 rows with 8 / 16 18.9 / 22.6).
+  constexpr int kAlone = 12288, kLong = 10240, kShort = 4096;
+  while (resident && C < kMaxCluster) {
+    const int turn = clusters_at_a_time(2 * C);
+    const int whole = C == 1 ? (a.R <= turn / 8 ? kAlone : kSlice) : (a.R <= turn / 4 ? kShort : kLong);
+    if (a.R > turn || slice_positions(a.V, C) <= whole) break;
+    C *= 2;
+  }
+  const int chunk = (slice_positions(a.V, C) + kWarps * kStep - 1) / (kWarps * kStep) * kStep;
+  const size_t smem = resident ? sizeof(Shared<kBinsResident>) + size_t(chunk) * kWarps * 4 : sizeof(Shared<kBinsStreamed>);
+  auto kernel = a.bf16 ? (resident ? sample_kernel<true, true> : sample_kernel<true, false>)
+                       : (resident ? sample_kernel<false, true> : sample_kernel<false, false>);
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = C;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // the kernel starts with pdl_wait()
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
+  cudaLaunchConfig_t cfg = cluster_config(a.R, C, smem, attr);
+  cfg.stream = stream;
   cfg.numAttrs = pdl_flag() ? 2 : 1;
   cuda_check(cudaLaunchKernelEx(&cfg, kernel, a, C, chunk), "sample_tokens launch");
 }
