@@ -24,9 +24,10 @@
 //
 // Measured on B200: one row of 129,280 FP32 logits with top-k and top-p 19 us
 // (its bytes take 0.1 us: the barriers and exchanges between CTAs are the
-// bound), 16 rows 29 us; 256 rows with top-p 198 us, streamed, against 20 us
-// for their bytes: bound by instruction issue (94 warp instructions per 32
-// logits; a quotient, two exponentials and two histogram additions each).
+// bound), 16 rows 29 us (32 us with a setting per row); 256 rows with top-p
+// 198 us, streamed, against 20 us for their bytes: bound by instruction issue
+// (94 warp instructions per 32 logits; a quotient, two exponentials and two
+// histogram additions each) and by load latency.
 #include <algorithm>
 #include <atomic>
 #include <cmath>

@@ -50,10 +50,11 @@
 // keys 78 us with a cold L2, 2 x 128 rows over 64 keys 8 us.  A tile takes
 // 1,520 cycles per pair; the bound is the shared-memory reads of QK's operands
 // (N = 64 re-reads Q for every 64 keys: ~860 cycles a tile, PV ~600), next to
-// it the L2-to-SM path.  QK of two tiles at once (N = 128) reads Q half as often,
-// but has to wait for both tiles' records, and is slower: 260 against 229 us.  A record stage is held ~6,200 cycles from its load to
-// its PV, so four stages are needed to keep that pace: they fit because half of
-// P lies in the stage's RoPE chunk.  With three stages a tile took 2,080 cycles.
+// it the L2-to-SM path.  QK of two tiles at once (N = 128) reads Q half as
+// often, but has to wait for both tiles' records, and is slower: 260 against
+// 229 us.  A record stage is held ~6,200 cycles from its load to its PV, so four
+// stages are needed to keep that pace: they fit because half of P lies in the
+// stage's RoPE chunk.  With three stages a tile took 2,080 cycles.
 #include <algorithm>
 #include <vector>
 
@@ -755,15 +756,16 @@ __global__ void __launch_bounds__(DV / 4) prefix_mla_merge_kernel(const __grid_c
   const int64_t tail = mp.tail_row0 >= 0 ? mp.tail_row0 + row : -1;
   // Weights exp(lse_s - max) of up to 128 partials at a time (a row tile has at most one per SM pair): one
   // thread per partial, so that the partials' rows are then loaded without waiting for one another.  The first
-  // eight are on their way before the weights are known, and dropped where nothing was written (24 x 16 heads
-  // over 4,096 rows 19.8 -> 17.4 us; 16 of them in registers: 0.5 us slower at 8 x 2,032 rows).
+  // twelve are on their way before the weights are known, and dropped where nothing was written.  8 x 2,032 rows
+  // / 24 x 16 heads over 4,096 rows take 18.5 / 19.8 us with none ahead, 16.3 / 17.3 with eight, 15.6 / 16.5 with
+  // twelve; more registers then cost what the loads gain (8 x 2,032 rows 0.4 us slower with 16 than with eight).
   __shared__ float weight[DV / 4], red[2][4];
   const int n = s1 - s0 + (tail >= 0 ? 1 : 0);
   auto partial = [&](int k) { return k < s1 - s0 ? int64_t(s0 + k) * BM + lane : tail; };
   float lse = -INFINITY;
   if (int(threadIdx.x) < n) lse = part_lse[partial(int(threadIdx.x))];
   auto load = [&](int k) { return *reinterpret_cast<const float4*>(part_o + partial(k) * DV + d0); };
-  constexpr int kFirst = 8;
+  constexpr int kFirst = 12;
   float4 first[kFirst];
 #pragma unroll
   for (int k = 0; k < kFirst; ++k)
