@@ -548,6 +548,35 @@ def test_shared_prefix_mla_many_queries(B, T, H, P, S):
 
 
 @gpu
+@pytest.mark.parametrize("B,T,H,P,S", [
+    (1, 1, 128, 4100, 3),    # one row tile over more shares than the merge loads ahead
+    (2, 1, 16, 4100, 1),     # its tails next to the shares
+    (30, 1, 16, 2100, 9),    # several row tiles, a tail per query
+    (40, 2, 20, 700, 70),    # more tails than pairs
+    (9, 1, 128, 1990, 40),   # shares that straddle row tiles
+    (76, 1, 128, 520, 5),    # a whole wave, then shares
+])
+def test_shared_prefix_mla_shares(B, T, H, P, S):
+    q, prefix, tail = prefix_inputs(B, T, H, P, S, "cuda", seed=14)
+    lens = torch.randint(0, S + 1, (B,), generator=torch.Generator().manual_seed(15))
+    out, lse = ops.shared_prefix_mla(q, prefix, tail, lens.int().cuda(), SCALE, return_lse=True)
+    keep = sorted({0, B // 2, B - 1})
+    check_prefix(q[keep], prefix, tail[keep], lens[keep].tolist(), out[keep], lse[keep])
+
+
+@gpu
+@pytest.mark.parametrize("V", [12290, 18673, 50021])
+@pytest.mark.parametrize("R", [7, 15, 34, 72])
+def test_sample_does_not_depend_on_the_batch(V, R):
+    """Row counts that change how many CTAs a row has: the same draws as row by row."""
+    x, u = rows(R, V, seed=16)
+    got = ops.sample_tokens(x, u, temperature=0.9, top_k=400, top_p=0.9)
+    one = [ops.sample_tokens(x[r:r + 1], u[r:r + 1], temperature=0.9, top_k=400, top_p=0.9) for r in range(R)]
+    assert torch.equal(got[0], torch.cat([t for t, _ in one]))
+    assert torch.equal(got[1], torch.cat([p for _, p in one]))
+
+
+@gpu
 def test_sample_offsets_past_32_bits():
     x, u = rows(3, 5000, seed=11, dtype=torch.bfloat16)
     want = ops.sample_tokens(x, u, top_k=50)
